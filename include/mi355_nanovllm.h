@@ -1065,6 +1065,65 @@ uint64_t mi_xxh64_chain(const void* data, size_t len, int has_prefix, uint64_t p
 int mi_xxh64_chain_blocks(const int64_t* tokens, int n_blocks, int block_size, int has_prefix,
                           uint64_t prefix, uint64_t* out);
 
+/* ---- attention mass and eviction (fragment-native cache; no counterpart in the reference) -----------------------------
+ * The mass of a cached token is the softmax weight it has been given, summed over the query heads of its kv head:
+ *   mass [mass_rows][n_kv_heads][mass_len] fp32, one row per sequence, slot j of the row = slot j of the sequence's context.
+ * slots [batch] names the row that is read, slots_out [batch] the one that is written (the same one, or a row that no sequence of
+ * the call reads: a step that may be taken back leaves the old row).  A sequence whose row of slots_out is outside
+ * [0, mass_rows) has no mass written; one whose row of slots is there has a mass of 0 so far.  The tokens that a step itself stored
+ * have their mass set by it, older ones are added to, so a row needs no clearing when a sequence gets it; slots at or behind the
+ * context are left as they are.  No sums are made with atomics: the same call gives the same bits.
+ *
+ * Other than the entry points above, these look at block ids: a table entry outside [0, num_blocks) is a page that is not there -
+ * its tokens are masked (they get no weight), and nothing is copied from or to it.  What masked places of the cache hold (the rest of
+ * a page, stale values, NaN) reaches no result.  Tables are [rows][table_stride], of which table_width entries may be used;
+ * contexts are taken to be no longer than table_width * block_size.  head_dim 64 or 128, n_q_heads / n_kv_heads up to 16. */
+
+/* Bytes of workspace of mi_paged_attn_decode_mass: the scores (4 bytes a query head and token that the table has room for), and the splits'
+ * sums.  Contents need not be kept or cleared. */
+size_t mi_paged_attn_decode_mass_workspace(int batch, int n_q_heads, int n_kv_heads, int head_dim, int block_size, int table_width);
+
+/* mi_paged_attn_decode that also adds each token's weights of this step to its mass (the newest token's, slot context_len - 1, is
+ * set).  Rows with context_len <= 0, or without a page, produce zeros. */
+int mi_paged_attn_decode_mass(const mi_bf16* q, int64_t q_row_stride, const mi_bf16* k_cache, const mi_bf16* v_cache,
+                              int64_t num_blocks, const int32_t* block_table, int64_t table_stride, int table_width,
+                              const int32_t* context_lens, float* mass, int64_t mass_rows, int64_t mass_len, const int32_t* slots,
+                              const int32_t* slots_out, mi_bf16* out, void* workspace, size_t ws_bytes, int batch, int n_q_heads,
+                              int n_kv_heads, int head_dim, int block_size, float scale, mi_stream stream);
+
+/* Bytes of workspace of mi_prompt_attn_mass for q of n_tokens rows. */
+size_t mi_prompt_attn_mass_workspace(int n_seqs, int64_t n_tokens, int max_seqlen_q, int window, int n_q_heads, int n_kv_heads, int head_dim,
+                                     int block_size, int table_width);
+
+/* The mass that prompt rows give: arguments as of mi_paged_attn_prefill (q [n_tokens, n_q_heads, head_dim], K of the step's tokens in
+ * the cache already, row i of a sequence at position kv_len - q_len + i); of each sequence's rows the last `window` are taken, all of them
+ * for window 0.  Rows of a sequence behind the first max_seqlen_q from its end are not. */
+int mi_prompt_attn_mass(const mi_bf16* q, int64_t q_row_stride, int64_t n_tokens, const mi_bf16* k_cache, int64_t num_blocks,
+                        const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* cu_seqlens_q,
+                        const int32_t* kv_lens, int n_seqs, int max_seqlen_q, int window, float* mass, int64_t mass_rows,
+                        int64_t mass_len, const int32_t* slots, const int32_t* slots_out, void* workspace, size_t ws_bytes,
+                        int n_q_heads, int n_kv_heads, int head_dim, int block_size, float scale, mi_stream stream);
+
+/* Bytes of workspace of mi_kv_cache_evict. */
+size_t mi_kv_cache_evict_workspace(int batch, int n_kv_heads, int keep, int block_size, int table_width);
+
+/* Contexts of more than `keep` tokens are cut to `keep`: each kv head keeps the tokens at positions below `sinks`, the `recent`
+ * newest, and of the others those of the largest mass (equal masses: the lower slot; NaN below everything; sinks + recent <= keep).
+ * Tokens kept below slot `keep` stay there; the n-th kept one from behind goes to the n-th place that became free.  K, V, mass and
+ * position move.  A token's position: origin[row][kv head][slot] for slots below evicted[row][0], slot + evicted[row][1] (the tokens
+ * dropped so far) behind; a fresh sequence starts with evicted = {0, 0}.  origin [mass_rows][n_kv_heads][mass_len],
+ * evicted [mass_rows][2].  context_lens_out [batch] (may be context_lens) receives the contexts' lengths now.
+ *
+ * block_table_out: the pages that receive the result (the same table: in place), at least ceil(min(keep, room) / block_size) entries a row.  A page that other
+ * sequences share is to be replaced by a page of the sequence's own there; an entry is the entry of block_table at the same place or a
+ * page that no sequence of the call reads or writes otherwise.  Shorter contexts are only copied where pages or rows differ.  A
+ * sequence with a row outside [0, mass_rows), or whose context is longer than mass_len or its table, is left as it is. */
+int mi_kv_cache_evict(mi_bf16* k_cache, mi_bf16* v_cache, int64_t num_blocks, const int32_t* block_table, int64_t table_stride,
+                      const int32_t* block_table_out, int64_t table_out_stride, int table_width, const int32_t* context_lens,
+                      int32_t* context_lens_out, float* mass, int32_t* origin, int32_t* evicted, int64_t mass_rows, int64_t mass_len,
+                      const int32_t* slots, const int32_t* slots_out, int keep, int sinks, int recent, void* workspace,
+                      size_t ws_bytes, int batch, int n_kv_heads, int head_dim, int block_size, mi_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

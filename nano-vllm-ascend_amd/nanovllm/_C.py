@@ -283,6 +283,15 @@ _SIGNATURES = {
     "mi_general_delta_state_elems": (c_int64, [c_int, c_int, c_int]),
     "mi_general_delta": (c_int, [_p, c_int64, c_int, c_int, c_int, c_int, _p, c_int64, _p, _p, _p, _p, c_int, c_int, c_int,
                                  c_int, c_int, _p, c_int64, _p]),
+    "mi_paged_attn_decode_mass_workspace": (c_size_t, [c_int] * 6),
+    "mi_paged_attn_decode_mass": (c_int, [_p, c_int64, _p, _p, c_int64, _p, c_int64, c_int, _p, _p, c_int64, c_int64, _p, _p, _p, _p,
+                                          c_size_t, c_int, c_int, c_int, c_int, c_int, c_float, _p]),
+    "mi_prompt_attn_mass_workspace": (c_size_t, [c_int, c_int64, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "mi_prompt_attn_mass": (c_int, [_p, c_int64, c_int64, _p, c_int64, _p, c_int64, c_int, _p, _p, c_int, c_int, c_int, _p, c_int64, c_int64,
+                                    _p, _p, _p, c_size_t, c_int, c_int, c_int, c_int, c_float, _p]),
+    "mi_kv_cache_evict_workspace": (c_size_t, [c_int] * 5),
+    "mi_kv_cache_evict": (c_int, [_p, _p, c_int64, _p, c_int64, _p, c_int64, c_int, _p, _p, _p, _p, _p, c_int64, c_int64, _p, _p, c_int, c_int,
+                                  c_int, _p, c_size_t, c_int, c_int, c_int, c_int, _p]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -236,6 +236,161 @@ def paged_attn_prefill_fused(qkv, q_w, eps: float, positions, cos_sin, k_cache, 
     return out
 
 
+# --------------------------------------------------------------------------- attention mass, eviction by it
+def attn_mass_shape(rows: int, n_kv_heads: int, max_len: int) -> tuple[int, int, int]:
+    """Shape of one layer's mass (float32) and origin (int32): a row per sequence, a slot per cached token and kv head."""
+    return (rows, n_kv_heads, max_len)
+
+
+def _refuse(ok: bool, what: str) -> None:
+    if not ok:
+        raise _C.MiError(what)
+
+
+def _on_current_device(name: str, *tensors: torch.Tensor) -> None:
+    require_gpu(*tensors)
+    here = torch.cuda.current_device()
+    for t in tensors:
+        _refuse(t.device.index == here, f"{name}: a tensor on {t.device}, the current device is cuda:{here}")
+
+
+def _mass_operands(name: str, caches, tables, lens, slots, slots_out, states, n_kv_heads: int, block_size: int, others=()):
+    """The checks that the three operators share -> (batch, head_dim, slots_out, the first table's width and row stride)."""
+    n = lens.numel()
+    slots_out = slots if slots_out is None else slots_out
+    _on_current_device(name, *caches, *tables, lens, slots, slots_out, *states, *others)
+    for c in caches:
+        _refuse(c.dtype == _BF16 and c.is_contiguous() and c.dim() == 4 and c.shape == caches[0].shape,
+                f"{name}: caches are contiguous bfloat16 [blocks, kv heads, block_size / 16, 16 * head_dim]")
+    D = _head_dim_of(caches[0])
+    _refuse(D in (64, HEAD_DIM) and caches[0].shape[0] > 0 and block_size > 0 and block_size % 16 == 0
+            and caches[0].shape == kv_cache_shape(caches[0].shape[0], n_kv_heads, block_size, D),
+            f"{name}: a cache of shape {tuple(caches[0].shape)} for {n_kv_heads} kv heads and blocks of {block_size}")
+    for t in tables:
+        _refuse(t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] >= n and t.shape[1] > 0 and (t.stride(1) == 1 or t.shape[1] == 1)
+                and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]), f"{name}: block tables are int32 [sequences, blocks], a row's entries side by side")
+    for t in (lens, slots, slots_out):
+        _refuse(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.numel() == n,
+                f"{name}: lengths and slots are contiguous int32, one per sequence")
+    for t in states:
+        _refuse(t.dim() == 3 and t.is_contiguous() and t.shape == states[0].shape and t.shape[1] == n_kv_heads,
+                f"{name}: state rows are contiguous [rows, kv heads, slots]")
+    _refuse(states[0].dtype == _F32, f"{name}: the mass is float32")
+    width = tables[0].shape[1]
+    return n, D, slots_out, width, _table_stride(tables[0])
+
+
+def _table_stride(t) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _rows_of(name: str, q, width: int):
+    """q [rows, heads, head_dim] or [rows, heads * head_dim] as rows -> (rows, elements between them)"""
+    _refuse(q.dtype == _BF16 and q.dim() in (2, 3), f"{name}: q is bfloat16 [rows, heads, head_dim] or [rows, heads * head_dim]")
+    if q.dim() == 3:
+        _refuse(q.shape[1] * q.shape[2] == width and (q.stride(2) == 1 or q.shape[2] == 1) and (q.stride(1) == q.shape[2] or q.shape[1] == 1),
+                f"{name}: q of shape {tuple(q.shape)} with strides {q.stride()}")
+    else:
+        _refuse(q.shape[1] == width and q.stride(1) == 1, f"{name}: q of shape {tuple(q.shape)} with strides {q.stride()}")
+    stride = q.stride(0) if q.shape[0] > 1 else width
+    _refuse(q.numel() == 0 or (q.data_ptr() % 16 == 0 and stride % 8 == 0), f"{name}: rows of q start on 16 bytes")
+    return q.shape[0], stride
+
+
+def _mass_workspace(name: str, workspace, need: int, device):
+    if workspace is None:  # torch's allocator keeps it to the stream, or to the graph that is being captured
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    _refuse(workspace.is_contiguous() and workspace.device == device and workspace.numel() * workspace.element_size() >= need,
+            f"{name}: a contiguous workspace of {need} bytes on {device}")
+    return workspace
+
+
+def paged_attn_decode_mass(q, k_cache, v_cache, block_tables, context_lens, mass, slots, n_q_heads: int, n_kv_heads: int,
+                           block_size: int, scale: float, slots_out=None, out=None, workspace=None) -> torch.Tensor:
+    """paged_attn_decode that also keeps the tokens' attention mass: mass [rows, n_kv_heads, max_len] (float32; slots [batch] names
+    each sequence's row) grows by the softmax weights of this step, summed over the query heads of the kv head.  The newest token's
+    mass is set, so a row needs no clearing.  slots_out: rows that receive the result instead (slots: read only).
+    Block ids outside the cache mask their tokens.  A graph captures it with its own workspace."""
+    name = "paged_attn_decode_mass"
+    n, D, slots_out, width, stride = _mass_operands(name, (k_cache, v_cache), (block_tables,), context_lens, slots, slots_out, (mass,),
+                                                    n_kv_heads, block_size, (q,))
+    _refuse(n_q_heads > 0 and n_q_heads % n_kv_heads == 0 and n_q_heads // n_kv_heads <= 16,
+            f"{name}: {n_q_heads} query heads on {n_kv_heads} kv heads (up to 16 each)")
+    rows, q_stride = _rows_of(name, q, n_q_heads * D)
+    _refuse(rows == n, f"{name}: {rows} rows of q for {n} sequences")
+    if out is None:
+        out = torch.empty((n, n_q_heads * D), dtype=_BF16, device=q.device)
+    _refuse(out.dtype == _BF16 and out.is_contiguous() and out.numel() == n * n_q_heads * D and out.device == q.device,
+            f"{name}: out is contiguous bfloat16 [{n}, {n_q_heads * D}]")
+    if n == 0:
+        return out
+    ws = _mass_workspace(name, workspace, lib.mi_paged_attn_decode_mass_workspace(n, n_q_heads, n_kv_heads, D, block_size, width), q.device)
+    check(lib.mi_paged_attn_decode_mass(ptr(q), q_stride, ptr(k_cache), ptr(v_cache), k_cache.shape[0], ptr(block_tables), stride, width,
+                                        ptr(context_lens), ptr(mass), mass.shape[0], mass.shape[2], ptr(slots), ptr(slots_out), ptr(out), ptr(ws),
+                                        ws.numel() * ws.element_size(), n, n_q_heads, n_kv_heads, D, block_size, float(scale), stream()), name)
+    return out
+
+
+def prompt_attn_mass(q, k_cache, block_tables, cu_seqlens_q, kv_lens, max_seqlen_q: int, mass, slots, n_q_heads: int, n_kv_heads: int,
+                     block_size: int, scale: float, window: int = 0, slots_out=None, workspace=None) -> None:
+    """The attention mass that a prefill step's rows give (operands as paged_attn_prefill's; K of the step in the cache): all of a
+    sequence's rows, or its last `window`.  Tokens that the step stored have their mass set, those cached before are added to: portions
+    of a prompt follow one another, and decode steps follow them."""
+    name = "prompt_attn_mass"
+    n, D, slots_out, width, stride = _mass_operands(name, (k_cache,), (block_tables,), kv_lens, slots, slots_out, (mass,), n_kv_heads,
+                                                    block_size, (q, cu_seqlens_q))
+    _refuse(n_q_heads > 0 and n_q_heads % n_kv_heads == 0 and n_q_heads // n_kv_heads <= 16,
+            f"{name}: {n_q_heads} query heads on {n_kv_heads} kv heads (up to 16 each)")
+    rows, q_stride = _rows_of(name, q, n_q_heads * D)
+    _refuse(cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.is_contiguous() and cu_seqlens_q.numel() == n + 1,
+            f"{name}: cu_seqlens_q is contiguous int32, one more than the sequences")
+    _refuse(window >= 0 and max_seqlen_q >= 0, f"{name}: window {window}, max_seqlen_q {max_seqlen_q}")
+    if n == 0:
+        return
+    max_seqlen_q = min(int(max_seqlen_q), rows)
+    ws = _mass_workspace(name, workspace, lib.mi_prompt_attn_mass_workspace(n, rows, max(max_seqlen_q, 1), int(window), n_q_heads, n_kv_heads, D,
+                                                                            block_size, width), q.device)
+    check(lib.mi_prompt_attn_mass(ptr(q) if rows else ptr(k_cache), q_stride, rows, ptr(k_cache), k_cache.shape[0], ptr(block_tables), stride, width,
+                                  ptr(cu_seqlens_q), ptr(kv_lens), n, max_seqlen_q, int(window), ptr(mass), mass.shape[0], mass.shape[2],
+                                  ptr(slots), ptr(slots_out), ptr(ws), ws.numel() * ws.element_size(), n_q_heads, n_kv_heads, D, block_size,
+                                  float(scale), stream()), name)
+
+
+def kv_cache_evict(k_cache, v_cache, block_tables, context_lens, mass, origin, evicted, slots, keep: int, sinks: int, recent: int,
+                   block_size: int, block_tables_out=None, slots_out=None, context_lens_out=None, workspace=None) -> torch.Tensor:
+    """Cuts contexts of more than `keep` tokens to `keep`, in place: per kv head the tokens at positions below `sinks`, the `recent` newest
+    and those of the largest mass stay.  Kept tokens from slots behind `keep` move into the places that became free, K, V, mass and position
+    (origin, evicted: see mi_kv_cache_evict; a fresh sequence has evicted[row] = 0); what decodes next is stored at slot `keep`.  Returns the
+    contexts' lengths (context_lens_out, may be context_lens).
+
+    The pages that are written are the sequence's own: a page that other sequences share (a cached prefix) is replaced in
+    block_tables_out, which then receives what is kept.  slots_out likewise for the state's rows.  Head geometries of the plain cache layout
+    (attention_is_plain) are not served."""
+    name = "kv_cache_evict"
+    n_kv_heads = k_cache.shape[1] if k_cache.dim() == 4 else 0
+    tables = (block_tables,) if block_tables_out is None else (block_tables, block_tables_out)
+    if context_lens_out is None:
+        context_lens_out = torch.empty_like(context_lens)
+    n, D, slots_out, width, stride = _mass_operands(name, (k_cache, v_cache), tables, context_lens, slots, slots_out, (mass, origin),
+                                                    n_kv_heads, block_size, (evicted, context_lens_out))
+    _refuse(origin.dtype == torch.int32, f"{name}: origin is int32")
+    _refuse(evicted.dtype == torch.int32 and evicted.is_contiguous() and evicted.shape == (mass.shape[0], 2),
+            f"{name}: evicted is contiguous int32 [{mass.shape[0]}, 2]")
+    _refuse(context_lens_out.dtype == torch.int32 and context_lens_out.is_contiguous() and context_lens_out.shape == context_lens.shape,
+            f"{name}: context_lens_out is contiguous int32 [{n}]")
+    _refuse(keep > 0 and sinks >= 0 and recent >= 0 and sinks + recent <= keep,
+            f"{name}: {sinks} first and {recent} newest tokens of {keep} kept")
+    _refuse(tables[-1].shape[1] >= -(-min(keep, width * block_size) // block_size), f"{name}: block_tables_out has no room for {keep} tokens")
+    if n == 0:
+        return context_lens_out
+    ws = _mass_workspace(name, workspace, lib.mi_kv_cache_evict_workspace(n, n_kv_heads, int(keep), block_size, width), k_cache.device)
+    check(lib.mi_kv_cache_evict(ptr(k_cache), ptr(v_cache), k_cache.shape[0], ptr(block_tables), stride, ptr(tables[-1]),
+                                _table_stride(tables[-1]), width, ptr(context_lens), ptr(context_lens_out), ptr(mass), ptr(origin), ptr(evicted),
+                                mass.shape[0], mass.shape[2], ptr(slots), ptr(slots_out), int(keep), int(sinks), int(recent), ptr(ws),
+                                ws.numel() * ws.element_size(), n, n_kv_heads, D, block_size, stream()), name)
+    return context_lens_out
+
+
 # --------------------------------------------------------------------------- norms
 def rmsnorm(x, w, eps: float, out=None) -> torch.Tensor:
     """x: [rows, cols] (contiguous rows) or [T, H, cols] with arbitrary token stride."""
