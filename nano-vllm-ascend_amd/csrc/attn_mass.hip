@@ -23,17 +23,30 @@ struct Pages {
   int64_t table_stride;
   int64_t num_blocks;
   int tpb;        // 16-token tiles per block
+  int tpb_shift;  // log2 of it, -1 where it is no power of two
   int cap;        // tokens that a table row has room for
   int n_kv;
 };
 
-// element offset of tile t of (table row, kv head); `there`: the row names a block of the cache (reads go to block 0 otherwise)
+// an entry of a table, which no kernel here writes: by way of the constant address space a wave-uniform index is a scalar read, also behind stores
+__device__ __forceinline__ int32_t entry(const int32_t* row, int i) {
+  return reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(reinterpret_cast<uintptr_t>(row))[i];
+}
+__device__ __forceinline__ int block_of(const Pages& pg, int t) { return pg.tpb_shift >= 0 ? t >> pg.tpb_shift : t / pg.tpb; }
+// element offset of tile t of kv head h in block blk; `there`: that is a block of the cache (reads go to block 0 otherwise)
+template <int D>
+__device__ __forceinline__ int64_t tile_in(const Pages& pg, int32_t blk, int t, int h, bool& there) {
+  there = blk >= 0 && blk < pg.num_blocks;
+  return (((there ? (int64_t)blk : 0) * pg.n_kv + h) * pg.tpb + (t - block_of(pg, t) * pg.tpb)) * (16 * D);
+}
 template <int D>
 __device__ __forceinline__ int64_t tile_at(const Pages& pg, const int32_t* row, int t, int h, bool& there) {
-  const int bi = t / pg.tpb;
-  const int32_t blk = row[bi];
-  there = blk >= 0 && blk < pg.num_blocks;
-  return (((there ? (int64_t)blk : 0) * pg.n_kv + h) * pg.tpb + (t - bi * pg.tpb)) * (16 * D);
+  return tile_in<D>(pg, entry(row, block_of(pg, t)), t, h, there);
+}
+
+int tile_shift(int block_size) {
+  const int tpb = block_size / 16;
+  return (tpb & (tpb - 1)) == 0 ? __builtin_ctz(tpb) : -1;
 }
 
 struct MassRows {
@@ -340,9 +353,10 @@ struct PromptMass {
   MassRows rows;
   uint16_t* packed;  // [n_kv][tiles][D * 32] rows in operand order
   float* part_ml;    // [n_kv][parts][tiles * 32][2]
+  float* part_sum;   // [n_kv][row_parts][n_seqs][cap]
   float* lse;        // [n_kv][tiles * 32]: log2 of the row's sum of exp2, infinity for a row that sees nothing
   int64_t tiles;     // 32-row tiles of a kv head, all sequences
-  int n_tokens, window, max_rows, G, parts, row_waves;
+  int n_tokens, n_seqs, window, max_rows, G, parts, row_parts;
   float scale_log2e;
 };
 
@@ -367,119 +381,323 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptMass& a, int b) {
   return s;
 }
 
-// two page tiles of K as the A operand of 32x32x16: lane (half, t) has dims 16 j + 8 half .. + 7 of token t
-template <int D>
-__device__ __forceinline__ void load_keys(const uint16_t* kc, int64_t at0, int64_t at1, int lane, u32x4 (&K)[D / 16]) {
-  const uint16_t* p = kc + ((lane & 16) ? at1 : at0) + ((lane >> 5) * 16 + (lane & 15)) * 8;
-#pragma unroll
-  for (int j = 0; j < D / 16; ++j) K[j] = *reinterpret_cast<const u32x4*>(p + (j >> 1) * 512 + (j & 1) * 256);
-}
-
 // token of the 32 that register r of lane half `hf` holds
 __device__ __forceinline__ int key_of(int r, int hf) { return (r >> 2) * 8 + hf * 4 + (r & 3); }
 
-template <int D>
-__device__ __forceinline__ f32x16 products(const u32x4 (&K)[D / 16], const u32x4 (&Q)[D / 16]) {
-  f32x16 s = {};
+// A stream of 64-row pairs of tiles goes through three buffers in LDS, by way of registers: in step i pair i + 2 is written and pair i + 3
+// requested, so that the products of the next tile always run under the powers of this one.  (Copied to LDS without registers, a tile's reads wait
+// for every copy in flight: the compiler tells them apart by nothing but the array.)
+__device__ __forceinline__ void pair_done() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+__device__ __forceinline__ int after(int slot) { return slot == 2 ? 0 : slot + 1; }
+
+// One step: the products of the next tile (fragment j of the stream from LDS by two of the wave's own), and between the
+// matrix instructions, 32 cycles each and of two independent chains, what `power` does with score r of this tile's side t and `add` with what
+// came of it: 4 + 8 + 4 cycles for 32 scores, the time of the 16 (8) products.  A wave issues in order, so the order is written down here;
+// the compiler's own has the products of a chain behind one another, each waiting for the last.
+template <int J, typename Read, typename Multiply, typename Power, typename Add>
+__device__ __forceinline__ void multiply_among(Read&& read, Multiply&& multiply, Power&& power, Add&& add) {
+  constexpr int N = 32 / (2 * J);  // scores a matrix instruction
+  constexpr int AHEAD = 4;         // fragments on their way from LDS
+  u32x4 f[J];
 #pragma unroll
-  for (int j = 0; j < D / 16; ++j) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(K[j]), as_frag(Q[j]), s, 0, 0, 0);
-  return s;
+  for (int j = 0; j < AHEAD; ++j) f[j] = read(j);
+  float e[N];
+  __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+  for (int i = 0; i < 2 * J; ++i) {
+    float was[N];
+#pragma unroll
+    for (int v = 0; v < N; ++v) was[v] = e[v];
+#pragma unroll
+    for (int v = 0; v < N; ++v) e[v] = power((i * N + v) >> 4, (i * N + v) & 15);
+#pragma unroll
+    for (int v = 0; v < N; ++v)
+      if (i > 0) add(((i - 1) * N + v) >> 4, ((i - 1) * N + v) & 15, was[v]);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(i & 1, i >> 1, f[i >> 1]);
+    if ((i & 1) && (i >> 1) + AHEAD < J) f[(i >> 1) + AHEAD] = read((i >> 1) + AHEAD);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+#pragma unroll
+  for (int v = 0; v < N; ++v) add(((2 * J - 1) * N + v) >> 4, ((2 * J - 1) * N + v) & 15, e[v]);
 }
 
-// A wave: 64 rows, one part of the keys they see.  grid (kv heads, row blocks x key blocks, sequences)
+// ---- the row sums: a wave's 64 rows, two tiles of 32
+template <int D>
+struct RowTiles {
+  static constexpr int J = D / 16;
+  u32x4 Q[2][J];
+  int limit[2];                      // keys that the lane's row sees
+  float m[2], shift[2], l[2];        // reference point, what is added to a score (its negative; infinity before there is one), sum
+  int64_t tile;
+  bool second;                       // the second tile is there
+  int all, most;                     // keys that every row sees, that the last one sees
+
+  // rows group * 64 on; group -1: none
+  __device__ __forceinline__ void load(const PromptMass& a, const PromptSeq& sq, int h, int group, int lane, bool pack) {
+    const int hf = lane >> 5;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int r = group * 64 + t * 32 + (lane & 31);
+      const bool on = group >= 0 && r < sq.n_rows;
+      const int token = on ? r / a.G : 0;
+      limit[t] = on ? min(sq.first + token + 1, sq.kv) : 0;
+      const uint16_t* p = a.q + (int64_t)(sq.q_begin + token) * a.q_stride + (int64_t)(h * a.G + (on ? r - token * a.G : 0)) * D + 8 * hf;
+#pragma unroll
+      for (int j = 0; j < J; ++j) Q[t][j] = on ? *reinterpret_cast<const u32x4*>(p + 16 * j) : u32x4{0, 0, 0, 0};
+      m[t] = -INFINITY, shift[t] = INFINITY, l[t] = 0.f;
+    }
+    tile = sq.tile0 + group * 2;
+    second = group * 64 + 32 < sq.n_rows;
+    all = group >= 0 && group * 64 + 64 <= sq.n_rows ? min(sq.first + group * 64 / a.G + 1, sq.kv) : 0;
+    most = seen_by(a, sq, group);
+    if (pack && group >= 0) {
+      uint16_t* to = a.packed + (h * a.tiles + tile) * (32 * D) + lane * 8;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (t == 0 || second)
+#pragma unroll
+          for (int j = 0; j < J; ++j) *reinterpret_cast<u32x4*>(to + t * (32 * D) + j * 512) = Q[t][j];
+    }
+  }
+  static __device__ __forceinline__ int seen_by(const PromptMass& a, const PromptSeq& sq, int group) {
+    return group < 0 ? 0 : max(min(sq.first + min(group * 64 + 63, sq.n_rows - 1) / a.G + 1, sq.kv), 0);
+  }
+  // The reference point only has to be near the maximum (32 bits hold sums of up to 2^8 as they do those of up to 1), and a sum of 16 powers tells
+  // whether it is: no maximum is taken while the sums stay below.  Infinite until a key was seen, so that the first one comes here.
+  __device__ __forceinline__ float move_to(int t, float mx) {
+    const float mn = fmaxf(m[t], mx), to = mn == -INFINITY ? 0.f : -mn;
+    l[t] *= __builtin_amdgcn_exp2f(m[t] + to);
+    m[t] = mn;
+    shift[t] = mn == -INFINITY ? INFINITY : -mn;
+    return to;
+  }
+  __device__ __forceinline__ void add_plain(int t, const f32x16& s, float now, float scale) {
+    if (__any(!(now <= 256.f))) {
+      float mx = -INFINITY, part[4] = {};
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[r] * scale);
+      const float to = move_to(t, mx);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) part[r & 3] += __builtin_amdgcn_exp2f(fmaf(s[r], scale, to));
+      now = (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    l[t] += now;
+  }
+  __device__ __forceinline__ void multiply(const u32x4 (&K)[J], f32x16 (&s)[2]) const {
+    s[0] = f32x16{};
+    s[1] = f32x16{};
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(K[j]), as_frag(Q[0][j]), s[0], 0, 0, 0);
+      s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(K[j]), as_frag(Q[1][j]), s[1], 0, 0, 0);
+    }
+  }
+  // key tile k, of which rows see a part or whose pages may not be there
+  __device__ __forceinline__ void add_masked(const f32x16 (&s)[2], int k, int hf, bool there0, bool there1, float scale) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      auto seen = [&](int r) { return (32 * k + key_of(r, hf) < limit[t]) & (r < 8 ? there0 : there1); };
+      float mx = -INFINITY, part[4] = {};
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, seen(r) ? s[t][r] * scale : -INFINITY);
+      const float to = move_to(t, mx);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float e = __builtin_amdgcn_exp2f(fmaf(s[t][r], scale, to));
+        part[r & 3] += seen(r) ? e : 0.f;
+      }
+      l[t] += (part[0] + part[1]) + (part[2] + part[3]);
+    }
+  }
+  __device__ __forceinline__ void store(const PromptMass& a, int h, int part, int lane) const {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float mo = __shfl_xor(m[t], 32, 64), lo = __shfl_xor(l[t], 32, 64);
+      const float M = fmaxf(m[t], mo), to = M == -INFINITY ? 0.f : -M;
+      const float L = l[t] * __builtin_amdgcn_exp2f(m[t] + to) + lo * __builtin_amdgcn_exp2f(mo + to);
+      const int64_t at = (tile + t) * 32 + (lane & 31);
+      if (lane < 32 && (t == 0 || second)) {
+        if (a.parts == 1) {
+          a.lse[h * a.tiles * 32 + at] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
+        } else {
+          float* ml = a.part_ml + ((h * (int64_t)a.parts + part) * a.tiles * 32 + at) * 2;
+          ml[0] = M;
+          ml[1] = L;
+        }
+      }
+    }
+  }
+};
+
+// Many rows: a workgroup's four waves have 64 each and share a stream of keys.
+// grid (kv heads, row blocks x parts of the keys, sequences)
 template <int D>
 __global__ __launch_bounds__(256, 2) void prompt_rows_kernel(PromptMass a) {
+  constexpr int J = D / 16, PIECES = D / 64, TILE = 32 * D;  // 1 KiB pieces of a tile that a wave copies
+  __shared__ __attribute__((aligned(16))) uint16_t stage[3][2 * TILE];
+  const int h = blockIdx.x, b = blockIdx.z;
+  const PromptSeq sq = prompt_seq(a, b);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hf = lane >> 5;
+  const int part = blockIdx.y % a.parts;
+  // the rows that see most first
+  const int last_group = ((sq.n_rows + 63) >> 6) - 1 - (int)(blockIdx.y / a.parts) * 4, group = last_group - wave;
+  if (last_group < 0) return;  // uniform for the workgroup; a wave without rows of its own still copies
+  RowTiles<D> x;
+  x.load(a, sq, h, group, lane, part == 0);
+  // pairs of 32-key tiles
+  const int pairs = (RowTiles<D>::seen_by(a, sq, last_group) + 63) >> 6, share = (pairs + a.parts - 1) / a.parts;
+  const int k0 = part * share, k1 = min(k0 + share, (x.most + 63) >> 6);
+  const int32_t* row = a.pg.table + (int64_t)b * a.pg.table_stride;
+  const int last_tile = max((sq.kv + 15) / 16 - 1, 0);
+  bool holes = false;  // a page of the part is not there
+  for (int t = 4 * k0 + lane; t < min(4 * (k0 + share), last_tile + 1); t += 64) {
+    bool there;
+    tile_in<D>(a.pg, row[block_of(a.pg, t)], t, h, there);
+    holes |= !there;
+  }
+  holes = __any(holes);
+
+  // this wave's part of the stream's next pair (a 16-token page tile of each 32, half of it), and the ids of the blocks behind that: a table entry is
+  // read a step before the address that needs it
+  u32x4 next[2][PIECES];
+  int32_t ids[2];
+  auto page_tile = [&](int k, int i) { return min(4 * k + 2 * i + (wave >> 1), last_tile); };
+  auto look_up = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ids[i] = entry(row, block_of(a.pg, page_tile(k, i)));
+  };
+  auto request = [&](int k) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      bool there;
+      const uint16_t* p = a.kc + tile_in<D>(a.pg, ids[i], page_tile(k, i), h, there) + (wave & 1) * PIECES * 512 + lane * 8;
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j) next[i][j] = *reinterpret_cast<const u32x4*>(p + j * 512);
+    }
+    look_up(k + 1);
+  };
+  auto put = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < PIECES; ++j) *reinterpret_cast<u32x4*>(&stage[slot][i * TILE + (wave * PIECES + j) * 512 + lane * 8]) = next[i][j];
+  };
+  const uint16_t* const keys = &stage[0][(lane & 16 ? 16 * D : 0) + (hf * 16 + (lane & 15)) * 8];
+  auto fragment = [&](int slot, int i, int j) __attribute__((always_inline)) {
+    return *reinterpret_cast<const u32x4*>(keys + slot * (2 * TILE) + i * TILE + (j >> 1) * 512 + (j & 1) * 256);
+  };
+  auto multiply = [&](int slot, int i, f32x16 (&s)[2]) __attribute__((always_inline)) {
+    u32x4 K[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) K[j] = fragment(slot, i, j);
+    x.multiply(K, s);
+  };
+  // a tile that all rows see whole: its powers, with the products of the next one (tile i of the pair in next_slot) among them
+  auto step_plain = [&](const f32x16 (&s)[2], f32x16 (&next_s)[2], int next_slot, int i) __attribute__((always_inline)) {
+    float sum[2][4];
+    multiply_among<J>([&](int j) { return fragment(next_slot, i, j); },
+                      [&](int t, int j, const u32x4& K) {
+                        next_s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(K), as_frag(x.Q[t][j]), j == 0 ? f32x16{} : next_s[t], 0, 0, 0);
+                      },
+                      [&](int t, int r) { return __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale_log2e, x.shift[t])); },
+                      [&](int t, int r, float e) { sum[t][r & 3] = r < 4 ? e : sum[t][r & 3] + e; });
+#pragma unroll
+    for (int t = 0; t < 2; ++t) x.add_plain(t, s[t], (sum[t][0] + sum[t][1]) + (sum[t][2] + sum[t][3]), a.scale_log2e);
+  };
+  if (share > 0) {
+    int k = k0, at = 0, to = 2;  // pair k's buffer, pair k + 2's
+    auto advance = [&]() __attribute__((always_inline)) {
+      put(to);
+      request(k + 3);
+    };
+    auto done = [&]() __attribute__((always_inline)) {
+      pair_done();
+      ++k;
+      at = after(at);
+      to = after(to);
+    };
+    look_up(k0);
+    request(k0);
+    put(0);
+    request(k0 + 1);
+    put(1);
+    request(k0 + 2);
+    pair_done();
+    const int plain = holes ? k0 : max(min(x.all >> 6, k1), k0);
+    if (k < plain) {
+      f32x16 s[2][2];
+      multiply(at, 0, s[0]);
+      do {
+        advance();
+        step_plain(s[0], s[1], at, 1);
+        step_plain(s[1], s[0], after(at), 0);
+        done();
+      } while (k < plain);
+    }
+    while (k < k0 + share) {
+      advance();
+      if (k < k1) {
+#pragma unroll 1
+        for (int i = 0; i < 2; ++i) {
+          f32x16 s[2];
+          multiply(at, i, s);
+          bool there0, there1;
+          tile_at<D>(a.pg, row, min(4 * k + 2 * i, last_tile), h, there0);
+          tile_at<D>(a.pg, row, min(4 * k + 2 * i + 1, last_tile), h, there1);
+          x.add_masked(s, 2 * k + i, hf, there0, there1, a.scale_log2e);
+        }
+      }
+      done();
+    }
+  }
+  if (group >= 0) x.store(a, h, part, lane);
+}
+
+// Few rows (up to 192 of a sequence and kv head): nothing to share a stream of keys with.  A wave has 64 rows and a part of the keys, whose fragments
+// come straight from the cache, a tile ahead.  grid (kv heads, row groups x blocks of 4 parts, sequences)
+template <int D>
+__global__ __launch_bounds__(256, 2) void prompt_few_rows_kernel(PromptMass a) {
   constexpr int J = D / 16;
   const int h = blockIdx.x, b = blockIdx.z;
   const PromptSeq sq = prompt_seq(a, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hf = lane >> 5;
-  const int key_blocks = a.parts / (4 / a.row_waves);
-  const int part = (blockIdx.y % key_blocks) * (4 / a.row_waves) + wave / a.row_waves;
-  const int groups = (sq.n_rows + 63) >> 6;
-  // the rows that see most first
-  const int group = groups - 1 - ((blockIdx.y / key_blocks) * a.row_waves + wave % a.row_waves);
-  if (group < 0) return;
-
-  u32x4 Q[2][J];
-  int limit[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int r = group * 64 + t * 32 + (lane & 31);
-    const bool on = r < sq.n_rows;
-    const int token = r / a.G;
-    limit[t] = on ? min(sq.first + token + 1, sq.kv) : 0;
-    const uint16_t* p = a.q + (int64_t)(sq.q_begin + token) * a.q_stride + (int64_t)(h * a.G + r - token * a.G) * D + 8 * hf;
-#pragma unroll
-    for (int j = 0; j < J; ++j) Q[t][j] = on ? *reinterpret_cast<const u32x4*>(p + 16 * j) : u32x4{0, 0, 0, 0};
-  }
-  const int64_t tile = sq.tile0 + group * 2;
-  const bool second = group * 64 + 32 < sq.n_rows;  // the group's second tile is there
-  if (part == 0) {
-    uint16_t* to = a.packed + (h * a.tiles + tile) * (32 * D) + lane * 8;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-      if (t == 0 || second)
-#pragma unroll
-        for (int j = 0; j < J; ++j) *reinterpret_cast<u32x4*>(to + t * (32 * D) + j * 512) = Q[t][j];
-  }
-  // what every row sees, what the last one does
-  const int all = min(sq.first + group * 64 / a.G + 1, sq.kv);
-  const int most = min(sq.first + min(group * 64 + 63, sq.n_rows - 1) / a.G + 1, sq.kv);
-  const bool full = group * 64 + 64 <= sq.n_rows;
-  const int steps = (max(most, 0) + 31) >> 5, share = (steps + a.parts - 1) / a.parts;
-  const int k0 = min(part * share, steps), k1 = min(k0 + share, steps);
-  const int last_tile = max((sq.kv + 15) / 16 - 1, 0);
+  const int blocks = a.parts / 4, part = (blockIdx.y % blocks) * 4 + wave, group = blockIdx.y / blocks;
+  if (group * 64 >= sq.n_rows) return;
+  RowTiles<D> x;
+  x.load(a, sq, h, group, lane, part == 0);
+  const int tiles = (x.most + 31) >> 5, share = (tiles + a.parts - 1) / a.parts, k0 = part * share, k1 = min(k0 + share, tiles);
   const int32_t* row = a.pg.table + (int64_t)b * a.pg.table_stride;
-
-  float m[2] = {-INFINITY, -INFINITY}, shift[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
-  u32x4 K[J];
-  bool there0, there1;
-  auto load = [&](int k) __attribute__((always_inline)) {
-    const int64_t at0 = tile_at<D>(a.pg, row, min(2 * k, last_tile), h, there0), at1 = tile_at<D>(a.pg, row, min(2 * k + 1, last_tile), h, there1);
-    load_keys<D>(a.kc, at0, at1, lane, K);
+  const int last_tile = max((sq.kv + 15) / 16 - 1, 0);
+  struct Tile {
+    u32x4 K[J];
+    bool there0, there1;
   };
-  for (int k = k0; k < k1; ++k) {
-    load(k);
-    const bool plain = there0 && there1 && full && 32 * k + 32 <= all;
+  auto load = [&](int k, Tile& t) __attribute__((always_inline)) {
+    const int64_t at0 = tile_at<D>(a.pg, row, min(2 * k, last_tile), h, t.there0);
+    const int64_t at1 = tile_at<D>(a.pg, row, min(2 * k + 1, last_tile), h, t.there1);
+    const uint16_t* p = a.kc + ((lane & 16) ? at1 : at0) + (hf * 16 + (lane & 15)) * 8;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      f32x16 s = products<D>(K, Q[t]);
-      s *= a.scale_log2e;
-      if (!plain) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (32 * k + key_of(r, hf) >= limit[t] || !(r < 8 ? there0 : there1)) s[r] = -INFINITY;
-      }
-      float mx = s[0];
-#pragma unroll
-      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-      // the reference point only has to be near the maximum: sums of exp2 up to 2^8 keep their bits as those up to 1 do
-      if (__any(mx > m[t] + 8.f)) {
-        const float mn = fmaxf(m[t], mx), to = mn == -INFINITY ? 0.f : -mn;
-        l[t] *= __builtin_amdgcn_exp2f(m[t] + to);
-        m[t] = mn;
-        shift[t] = to;
-      }
-#pragma unroll
-      for (int r = 0; r < 16; ++r) l[t] += __builtin_amdgcn_exp2f(s[r] + shift[t]);
+    for (int j = 0; j < J; ++j) t.K[j] = *reinterpret_cast<const u32x4*>(p + (j >> 1) * 512 + (j & 1) * 256);
+  };
+  auto add = [&](int k, const Tile& t) __attribute__((always_inline)) {
+    f32x16 s[2];
+    x.multiply(t.K, s);
+    x.add_masked(s, k, hf, t.there0, t.there1, a.scale_log2e);
+  };
+  if (k0 < k1) {
+    Tile A, B;
+    load(k0, A);
+    for (int k = k0;; k += 2) {
+      load(min(k + 1, k1 - 1), B);
+      add(k, A);
+      if (k + 1 >= k1) break;
+      load(min(k + 2, k1 - 1), A);
+      add(k + 1, B);
+      if (k + 2 >= k1) break;
     }
   }
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const float mo = __shfl_xor(m[t], 32, 64), lo = __shfl_xor(l[t], 32, 64);
-    const float M = fmaxf(m[t], mo), to = M == -INFINITY ? 0.f : -M;
-    const float L = l[t] * __builtin_amdgcn_exp2f(m[t] + to) + lo * __builtin_amdgcn_exp2f(mo + to);
-    const int64_t at = (tile + t) * 32 + (lane & 31);
-    if (hf == 0 && (t == 0 || second)) {
-      if (a.parts == 1) {
-        a.lse[h * a.tiles * 32 + at] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
-      } else {
-        float* ml = a.part_ml + ((h * (int64_t)a.parts + part) * a.tiles * 32 + at) * 2;
-        ml[0] = M;
-        ml[1] = L;
-      }
-    }
-  }
+  x.store(a, h, part, lane);
 }
 
 __global__ __launch_bounds__(256) void prompt_join_kernel(PromptMass a) {
@@ -488,63 +706,152 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptMass a) {
   const int r = blockIdx.y * 256 + threadIdx.x;
   if (r >= ((sq.n_rows + 31) & ~31)) return;
   const int64_t at = sq.tile0 * 32 + r;
+  const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + h * (int64_t)a.parts * a.tiles * 32 + at;
   float M = -INFINITY, L = 0.f;
-  for (int p = 0; p < a.parts; ++p) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + ((h * (int64_t)a.parts + p) * a.tiles * 32 + at) * 2);
-    const float mn = fmaxf(M, ml.x), to = mn == -INFINITY ? 0.f : -mn;
-    L = L * __builtin_amdgcn_exp2f(M + to) + ml.y * __builtin_amdgcn_exp2f(ml.x + to);
+  for (int p = 0; p < a.parts; p += 8) {
+    float2 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = p + i < a.parts ? ml[(p + i) * a.tiles * 32] : float2{-INFINITY, 0.f};
+    float mn = M;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) mn = fmaxf(mn, v[i].x);
+    const float to = mn == -INFINITY ? 0.f : -mn;
+    L *= __builtin_amdgcn_exp2f(M + to);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) L += v[i].y * __builtin_amdgcn_exp2f(v[i].x + to);
     M = mn;
   }
   a.lse[h * a.tiles * 32 + at] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
 }
 
-// A wave: 64 keys, all rows that see one of them.  grid (kv heads, blocks of 256 keys, sequences)
+// The column sums.  A wave: 64 keys; the workgroup's 256 share a stream of the rows that see one of them, or of a part of those.
+// grid (kv heads, key blocks x row parts, sequences)
 template <int D>
 __global__ __launch_bounds__(256, 2) void prompt_columns_kernel(PromptMass a) {
-  constexpr int J = D / 16;
+  constexpr int J = D / 16, TILE = 32 * D, PIECES = D / 64;
+  __shared__ __attribute__((aligned(16))) uint16_t stage[3][2 * TILE];
   __shared__ float sm[4][64];
   const int h = blockIdx.x, b = blockIdx.z;
   const PromptSeq sq = prompt_seq(a, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hf = lane >> 5;
-  const int key0 = (blockIdx.y * 4 + wave) * 64;
-  if (key0 >= sq.kv) return;
+  const int key_blocks = (a.pg.cap + 255) >> 8, block0 = (int)(blockIdx.y % key_blocks) * 256, row_part = blockIdx.y / key_blocks;
+  const int key0 = block0 + wave * 64;
+  if (block0 >= sq.kv) return;  // uniform for the workgroup
   const int32_t* row = a.pg.table + (int64_t)b * a.pg.table_stride;
   const int last_tile = (sq.kv + 15) / 16 - 1;
   u32x4 K[2][J];
   bool there[4];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
+    // 32 keys as the A operand: lane (half, t) has dims 16 j + 8 half .. + 7 of token t
     const int k = key0 / 16 + 2 * t;
     const int64_t at0 = tile_at<D>(a.pg, row, min(k, last_tile), h, there[2 * t]);
     const int64_t at1 = tile_at<D>(a.pg, row, min(k + 1, last_tile), h, there[2 * t + 1]);
-    load_keys<D>(a.kc, at0, at1, lane, K[t]);
+    const uint16_t* p = a.kc + ((lane & 16) ? at1 : at0) + (hf * 16 + (lane & 15)) * 8;
+#pragma unroll
+    for (int j = 0; j < J; ++j) K[t][j] = *reinterpret_cast<const u32x4*>(p + (j >> 1) * 512 + (j & 1) * 256);
   }
-  const bool whole = there[0] && there[1] && there[2] && there[3];
+  const bool whole = there[0] && there[1] && there[2] && there[3] && key0 + 64 <= sq.kv;
   f32x16 sum[2] = {{}, {}};
-  // the first row that sees key0
-  const int tiles = (sq.n_rows + 31) >> 5, from = max(key0 - sq.first, 0) * a.G >> 5;
-  for (int i = from; i < tiles; ++i) {
-    const uint16_t* p = a.packed + (h * a.tiles + sq.tile0 + i) * (32 * D) + lane * 8;
-    u32x4 Q[J];
+  // row tiles: from the first that has a row which sees the workgroup's (the wave's) first key; from the first all of whose rows see all of
+  // the wave's keys
+  const int tiles = (sq.n_rows + 31) >> 5;
+  auto sees = [&](int key) { return (int)min((int64_t)max(key - sq.first, 0) * a.G, (int64_t)sq.n_rows); };
+  const int first = sees(block0) >> 5, share = (max(tiles - first, 0) + a.row_parts - 1) / a.row_parts;
+  const int i0 = min(first + row_part * share, tiles), i1 = min(i0 + share, tiles);
+  const int wave_first = key0 < sq.kv ? sees(key0) >> 5 : tiles, plain_from = whole ? (sees(key0 + 63) + 31) >> 5 : tiles;
+  const uint16_t* const packed = a.packed + (h * a.tiles + sq.tile0) * TILE + wave * PIECES * 512 + lane * 8;
+  const float* const lses = a.lse + (h * a.tiles + sq.tile0) * 32 + (lane & 31);
+  u32x4 next[2][PIECES];
+  float lse[4][2];  // of the rows of pairs i .. i + 3
+  auto request = [&](int i) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < J; ++j) Q[j] = *reinterpret_cast<const u32x4*>(p + j * 512);
-    const float lse = a.lse[h * a.tiles * 32 + (sq.tile0 + i) * 32 + (lane & 31)];
-    const int limit = min(sq.first + (i * 32 + (lane & 31)) / a.G + 1, sq.kv);
-    const bool plain = whole && key0 + 64 <= min(sq.first + i * 32 / a.G + 1, sq.kv);
+    for (int u = 0; u < 2; ++u) {
+      const int t = min(i + u, i1 - 1);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const f32x16 s = products<D>(K[t], Q);
-      if (plain) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sum[t][r] += __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2e, -lse));
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[r], a.scale_log2e, -lse));
-          sum[t][r] += key0 + 32 * t + key_of(r, hf) < limit && there[2 * t + (r >> 3)] ? p : 0.f;
-        }
-      }
+      for (int p = 0; p < PIECES; ++p) next[u][p] = *reinterpret_cast<const u32x4*>(packed + (int64_t)t * TILE + p * 512);
+      lse[3][u] = lses[t * 32];
     }
+  };
+  auto put = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) *reinterpret_cast<u32x4*>(&stage[slot][u * TILE + (wave * PIECES + p) * 512 + lane * 8]) = next[u][p];
+      lse[0][u] = lse[1][u], lse[1][u] = lse[2][u], lse[2][u] = lse[3][u];
+    }
+  };
+  auto fragment = [&](int slot, int u, int j) __attribute__((always_inline)) {
+    return *reinterpret_cast<const u32x4*>(&stage[slot][u * TILE + j * 512 + lane * 8]);
+  };
+  auto multiply = [&](int slot, int u, f32x16 (&s)[2]) __attribute__((always_inline)) {
+    s[0] = f32x16{};
+    s[1] = f32x16{};
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const bf16x8 Q = as_frag(fragment(slot, u, j));
+      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(K[0][j]), Q, s[0], 0, 0, 0);
+      s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(K[1][j]), Q, s[1], 0, 0, 0);
+    }
+  };
+  // rows that all see the wave's keys (or none: their sum is infinite), with the products of the next ones (tile v of the pair in next_slot) among
+  // their powers
+  auto step_plain = [&](const f32x16 (&s)[2], float log_sum, f32x16 (&next_s)[2], int next_slot, int v) __attribute__((always_inline)) {
+    multiply_among<J>([&](int j) { return fragment(next_slot, v, j); },
+                      [&](int t, int j, const u32x4& Q) {
+                        next_s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(K[t][j]), as_frag(Q), j == 0 ? f32x16{} : next_s[t], 0, 0, 0);
+                      },
+                      [&](int t, int r) { return __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale_log2e, -log_sum)); },
+                      [&](int t, int r, float e) { sum[t][r] += e; });
+  };
+  auto step_masked = [&](int i, int slot, int u, float log_sum) __attribute__((always_inline)) {
+    f32x16 s[2];
+    multiply(slot, u, s);
+    const int rr = i * 32 + (lane & 31), limit = rr < sq.n_rows ? min(sq.first + rr / a.G + 1, sq.kv) : 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale_log2e, -log_sum));
+        sum[t][r] += ((key0 + 32 * t + key_of(r, hf) < limit) & there[2 * t + (r >> 3)]) ? p : 0.f;
+      }
+  };
+  if (i1 > i0) {
+    int i = i0, at = 0, to = 2;  // the pair of tiles i and i + 1, its buffer, that of the pair two further
+    auto advance = [&]() __attribute__((always_inline)) {
+      put(to);
+      request(i + 6);
+    };
+    auto done = [&]() __attribute__((always_inline)) {
+      pair_done();
+      i += 2;
+      at = after(at);
+      to = after(to);
+    };
+    auto masked = [&]() __attribute__((always_inline)) {
+      advance();
+      if (i >= wave_first) step_masked(i, at, 0, lse[0][0]);
+      if (i + 1 >= wave_first && i + 1 < i1) step_masked(i + 1, at, 1, lse[0][1]);
+      done();
+    };
+    request(i0);
+    put(0);
+    request(i0 + 2);
+    put(1);
+    request(i0 + 4);
+    pair_done();
+    while (i < min(plain_from, i1)) masked();
+    if (i + 2 <= i1) {
+      f32x16 s[2][2];
+      multiply(at, 0, s[0]);
+      do {
+        advance();
+        step_plain(s[0], lse[0][0], s[1], at, 1);
+        step_plain(s[1], lse[0][1], s[0], after(at), 0);
+        done();
+      } while (i + 2 <= i1);
+    }
+    if (i < i1) masked();
   }
 #pragma unroll
   for (int t = 0; t < 2; ++t)
@@ -558,17 +865,35 @@ __global__ __launch_bounds__(256, 2) void prompt_columns_kernel(PromptMass a) {
       if ((lane & 31) == 0) sm[wave][32 * t + key_of(r, hf)] = v;
     }
   __threadfence_block();  // (the wave's own part of the array)
+  const int j = key0 + lane;
+  if (j >= sq.kv) return;
+  const float v = sm[wave][lane];
+  if (a.row_parts > 1) {
+    a.part_sum[((int64_t)(h * a.row_parts + row_part) * a.n_seqs + b) * a.pg.cap + j] = v;
+    return;
+  }
   const float* had = a.rows.in(b, h);
   float* now = a.rows.out(b, h);
-  const int j = key0 + lane;
+  if (now != nullptr && j < a.rows.len) now[j] = (j < sq.fresh && had != nullptr ? had[j] : 0.f) + v;
+}
+
+__global__ __launch_bounds__(256) void prompt_add_kernel(PromptMass a) {
+  const int h = blockIdx.x, b = blockIdx.z, j = blockIdx.y * 256 + threadIdx.x;
+  const PromptSeq sq = prompt_seq(a, b);
+  const float* had = a.rows.in(b, h);
+  float* now = a.rows.out(b, h);
   if (now == nullptr || j >= sq.kv || j >= a.rows.len) return;
-  now[j] = (j < sq.fresh && had != nullptr ? had[j] : 0.f) + sm[wave][lane];
+  float v = 0.f;
+  for (int p = 0; p < a.row_parts; ++p) v += a.part_sum[((int64_t)(h * a.row_parts + p) * a.n_seqs + b) * a.pg.cap + j];
+  now[j] = (j < sq.fresh && had != nullptr ? had[j] : 0.f) + v;
 }
 
 struct PromptPlan {
-  int max_rows, row_waves, parts, groups;
+  int max_rows, parts, groups, row_parts;
+  bool few;
   int64_t tiles;
-  size_t packed, lse, ml;  // bytes
+  size_t packed, lse, ml, sum;  // bytes
+  size_t bytes() const { return packed + lse + ml + sum; }
 };
 
 PromptPlan prompt_plan(int n_seqs, int64_t n_tokens, int max_seqlen_q, int window, int n_q, int n_kv, int D, int64_t cap) {
@@ -577,15 +902,19 @@ PromptPlan prompt_plan(int n_seqs, int64_t n_tokens, int max_seqlen_q, int windo
   p.max_rows = window > 0 ? std::min(window, max_seqlen_q) : max_seqlen_q;
   p.tiles = window > 0 ? (int64_t)n_seqs * (((int64_t)p.max_rows * G + 31) / 32) : n_tokens * G / 32 + n_seqs;
   p.groups = (int)(((int64_t)p.max_rows * G + 63) / 64);
-  p.row_waves = p.groups >= 4 ? 4 : p.groups >= 2 ? 2 : 1;
-  const int key_waves = 4 / p.row_waves;
-  // parts of the keys until every SIMD has two waves, of 128 keys at least
-  const int64_t waves = (int64_t)n_seqs * n_kv * p.groups, want = (2048 + waves - 1) / std::max<int64_t>(waves, 1);
-  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>({want, (cap + 127) / 128, 64}));
-  p.parts = (int)((parts + key_waves - 1) / key_waves * key_waves);
+  p.few = p.groups <= 3;
+  const int64_t units = std::max<int64_t>((int64_t)n_seqs * n_kv, 1);
+  // parts of the keys until there are two workgroups a CU (few rows: waves, in fours), of 128 keys at least
+  const int64_t blocks = p.few ? units * p.groups : units * ((p.groups + 3) / 4);
+  const int64_t want = ((p.few ? 2048 : 512) + blocks - 1) / blocks, parts = std::max<int64_t>(1, std::min<int64_t>({want, (cap + 127) / 128, 64}));
+  p.parts = (int)(p.few ? (parts + 3) / 4 * 4 : parts);
+  // parts of the rows likewise, of eight tiles at least
+  const int64_t key_blocks = units * ((cap + 255) / 256);
+  p.row_parts = (int)std::max<int64_t>(1, std::min<int64_t>({1536 / key_blocks, (int64_t)p.groups / 4, 16}));
   p.packed = (size_t)n_kv * p.tiles * 32 * D * 2;
   p.lse = (size_t)n_kv * p.tiles * 32 * 4;
   p.ml = p.parts > 1 ? (size_t)n_kv * p.tiles * 32 * 8 * p.parts : 0;
+  p.sum = p.row_parts > 1 ? (size_t)n_kv * p.row_parts * n_seqs * cap * 4 : 0;
   return p;
 }
 
@@ -635,7 +964,7 @@ extern "C" int mi_paged_attn_decode_mass(const mi_bf16* q, int64_t q_row_stride,
   const size_t rows = (size_t)batch * n_q_heads;
   DecodeMass a;
   a.q = q, a.q_stride = q_row_stride, a.kc = k_cache, a.vc = v_cache;
-  a.pg = {block_table, table_stride, num_blocks, block_size / 16, (int)cap, n_kv_heads};
+  a.pg = {block_table, table_stride, num_blocks, block_size / 16, tile_shift(block_size), (int)cap, n_kv_heads};
   a.lens = context_lens;
   a.rows = {mass, mass_rows, mass_len, slots, slots_out, n_kv_heads};
   a.out = out;
@@ -657,10 +986,10 @@ extern "C" int mi_paged_attn_decode_mass(const mi_bf16* q, int64_t q_row_stride,
 
 extern "C" size_t mi_prompt_attn_mass_workspace(int n_seqs, int64_t n_tokens, int max_seqlen_q, int window, int n_q_heads, int n_kv_heads,
                                                 int head_dim, int block_size, int table_width) {
-  if (n_seqs <= 0 || n_tokens < 0 || max_seqlen_q <= 0 || n_kv_heads <= 0 || n_q_heads <= 0 || block_size <= 0 || table_width <= 0) return 0;
+  if (n_seqs <= 0 || n_tokens < 0 || max_seqlen_q < 0 || n_kv_heads <= 0 || n_q_heads <= 0 || block_size <= 0 || table_width <= 0) return 0;
   const PromptPlan p =
-      prompt_plan(n_seqs, n_tokens, max_seqlen_q, window, n_q_heads, n_kv_heads, head_dim, (int64_t)block_size * table_width);
-  return p.packed + p.lse + p.ml;
+      prompt_plan(n_seqs, n_tokens, std::max(max_seqlen_q, 1), window, n_q_heads, n_kv_heads, head_dim, (int64_t)block_size * table_width);
+  return p.bytes();
 }
 
 extern "C" int mi_prompt_attn_mass(const mi_bf16* q, int64_t q_row_stride, int64_t n_tokens, const mi_bf16* k_cache, int64_t num_blocks,
@@ -682,26 +1011,31 @@ extern "C" int mi_prompt_attn_mass(const mi_bf16* q, int64_t q_row_stride, int64
     return MI_EINVAL;
   if (!aligned16(q) || q_row_stride % 8 != 0 || !aligned16(k_cache) || !aligned16(workspace)) return MI_EINVAL;
   const PromptPlan p = prompt_plan(n_seqs, n_tokens, std::max(max_seqlen_q, 1), window, n_q_heads, n_kv_heads, head_dim, cap);
-  if (ws_bytes < p.packed + p.lse + p.ml) return MI_EWORKSPACE;
-  const int64_t row_blocks = (p.groups + p.row_waves - 1) / p.row_waves, key_blocks = p.parts / (4 / p.row_waves);
-  if (row_blocks * key_blocks > 65535 || (cap + 255) / 256 > 65535) return MI_EUNSUPPORTED;
+  if (ws_bytes < p.bytes()) return MI_EWORKSPACE;
+  const int64_t row_blocks = p.few ? (int64_t)p.groups * (p.parts / 4) : (int64_t)(p.groups + 3) / 4 * p.parts;
+  if (row_blocks > 65535 || (cap + 255) / 256 * p.row_parts > 65535) return MI_EUNSUPPORTED;
   PromptMass a;
   a.q = q, a.q_stride = q_row_stride, a.kc = k_cache;
-  a.pg = {block_table, table_stride, num_blocks, block_size / 16, (int)cap, n_kv_heads};
+  a.pg = {block_table, table_stride, num_blocks, block_size / 16, tile_shift(block_size), (int)cap, n_kv_heads};
   a.cu = cu_seqlens_q, a.kv_lens = kv_lens;
   a.rows = {mass, mass_rows, mass_len, slots, slots_out, n_kv_heads};
   char* ws = static_cast<char*>(workspace);
   a.packed = reinterpret_cast<uint16_t*>(ws);
   a.lse = reinterpret_cast<float*>(ws + p.packed);
   a.part_ml = reinterpret_cast<float*>(ws + p.packed + p.lse);
+  a.part_sum = reinterpret_cast<float*>(ws + p.packed + p.lse + p.ml);
   a.tiles = p.tiles;
-  a.n_tokens = (int)n_tokens, a.window = window, a.max_rows = std::min(p.max_rows, max_seqlen_q), a.G = G, a.parts = p.parts, a.row_waves = p.row_waves;
+  a.n_tokens = (int)n_tokens, a.window = window, a.max_rows = std::min(p.max_rows, max_seqlen_q), a.G = G, a.parts = p.parts, a.row_parts = p.row_parts, a.n_seqs = n_seqs;
   a.scale_log2e = scale * 1.44269504088896340736f;
-  const dim3 rg(n_kv_heads, (unsigned)(row_blocks * key_blocks), n_seqs), cg(n_kv_heads, (unsigned)((cap + 255) / 256), n_seqs);
-  if (head_dim == 128) prompt_rows_kernel<128><<<rg, 256, 0, S(stream)>>>(a);
+  const dim3 rg(n_kv_heads, (unsigned)row_blocks, n_seqs);
+  const dim3 cg(n_kv_heads, (unsigned)((cap + 255) / 256 * p.row_parts), n_seqs), ag(n_kv_heads, (unsigned)((cap + 255) / 256), n_seqs);
+  if (p.few && head_dim == 128) prompt_few_rows_kernel<128><<<rg, 256, 0, S(stream)>>>(a);
+  else if (p.few) prompt_few_rows_kernel<64><<<rg, 256, 0, S(stream)>>>(a);
+  else if (head_dim == 128) prompt_rows_kernel<128><<<rg, 256, 0, S(stream)>>>(a);
   else prompt_rows_kernel<64><<<rg, 256, 0, S(stream)>>>(a);
   if (p.parts > 1) prompt_join_kernel<<<dim3(n_kv_heads, (p.groups * 64 + 255) / 256, n_seqs), 256, 0, S(stream)>>>(a);
   if (head_dim == 128) prompt_columns_kernel<128><<<cg, 256, 0, S(stream)>>>(a);
   else prompt_columns_kernel<64><<<cg, 256, 0, S(stream)>>>(a);
+  if (p.row_parts > 1) prompt_add_kernel<<<ag, 256, 0, S(stream)>>>(a);
   return check_launch();
 }

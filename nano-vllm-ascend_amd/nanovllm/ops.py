@@ -242,67 +242,76 @@ def attn_mass_shape(rows: int, n_kv_heads: int, max_len: int) -> tuple[int, int,
     return (rows, n_kv_heads, max_len)
 
 
-def _refuse(ok: bool, what: str) -> None:
-    if not ok:
-        raise _C.MiError(what)
+def _refuse(name: str, what: str):
+    raise _C.MiError(f"{name}: {what}")
 
 
-def _on_current_device(name: str, *tensors: torch.Tensor) -> None:
-    require_gpu(*tensors)
-    here = torch.cuda.current_device()
+def _here(name: str, *tensors: torch.Tensor) -> int:
+    """the current device, which every one of the tensors is on"""
+    device = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
     for t in tensors:
-        _refuse(t.device.index == here, f"{name}: a tensor on {t.device}, the current device is cuda:{here}")
+        if t.get_device() != device or device < 0:
+            require_gpu(t)
+            _refuse(name, f"a tensor on {t.device}, the current device is cuda:{device}")
+    return device
 
 
-def _mass_operands(name: str, caches, tables, lens, slots, slots_out, states, n_kv_heads: int, block_size: int, others=()):
-    """The checks that the three operators share -> (batch, head_dim, slots_out, the first table's width and row stride)."""
-    n = lens.numel()
-    slots_out = slots if slots_out is None else slots_out
-    _on_current_device(name, *caches, *tables, lens, slots, slots_out, *states, *others)
-    for c in caches:
-        _refuse(c.dtype == _BF16 and c.is_contiguous() and c.dim() == 4 and c.shape == caches[0].shape,
-                f"{name}: caches are contiguous bfloat16 [blocks, kv heads, block_size / 16, 16 * head_dim]")
-    D = _head_dim_of(caches[0])
-    _refuse(D in (64, HEAD_DIM) and caches[0].shape[0] > 0 and block_size > 0 and block_size % 16 == 0
-            and caches[0].shape == kv_cache_shape(caches[0].shape[0], n_kv_heads, block_size, D),
-            f"{name}: a cache of shape {tuple(caches[0].shape)} for {n_kv_heads} kv heads and blocks of {block_size}")
-    for t in tables:
-        _refuse(t.dtype == torch.int32 and t.dim() == 2 and t.shape[0] >= n and t.shape[1] > 0 and (t.stride(1) == 1 or t.shape[1] == 1)
-                and (t.shape[0] == 1 or t.stride(0) >= t.shape[1]), f"{name}: block tables are int32 [sequences, blocks], a row's entries side by side")
-    for t in (lens, slots, slots_out):
-        _refuse(t.dtype == torch.int32 and t.dim() == 1 and t.is_contiguous() and t.numel() == n,
-                f"{name}: lengths and slots are contiguous int32, one per sequence")
-    for t in states:
-        _refuse(t.dim() == 3 and t.is_contiguous() and t.shape == states[0].shape and t.shape[1] == n_kv_heads,
-                f"{name}: state rows are contiguous [rows, kv heads, slots]")
-    _refuse(states[0].dtype == _F32, f"{name}: the mass is float32")
-    width = tables[0].shape[1]
-    return n, D, slots_out, width, _table_stride(tables[0])
+# (the checks' messages are put together only where one is raised: a decode step makes these calls per layer)
+def _cache_of(name: str, cache, n_kv_heads: int, block_size: int):
+    """one K or V cache of the fragment-native layout -> (blocks, head_dim)"""
+    if cache.dim() != 4 or cache.dtype is not _BF16 or not cache.is_contiguous():
+        _refuse(name, "caches are contiguous bfloat16 [blocks, kv heads, block_size / 16, 16 * head_dim]")
+    blocks, heads, tiles, elems = cache.shape
+    if blocks == 0 or heads != n_kv_heads or tiles <= 0 or tiles * 16 != block_size or (elems != 16 * HEAD_DIM and elems != 16 * 64):
+        _refuse(name, f"a cache of shape {tuple(cache.shape)} for {n_kv_heads} kv heads and blocks of {block_size}")
+    return blocks, elems // 16
 
 
-def _table_stride(t) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _table_of(name: str, table, n: int):
+    """block table -> (entries of a row, elements between rows)"""
+    if table.dim() != 2 or table.dtype is not torch.int32:
+        _refuse(name, "block tables are int32 [sequences, blocks]")
+    rows, width = table.shape
+    between, step = table.stride()
+    if rows < n or width == 0 or (step != 1 and width > 1) or (between < width and rows > 1):
+        _refuse(name, f"a block table of shape {tuple(table.shape)} with strides {table.stride()} for {n} sequences")
+    return width, between if rows > 1 else width
 
 
-def _rows_of(name: str, q, width: int):
-    """q [rows, heads, head_dim] or [rows, heads * head_dim] as rows -> (rows, elements between them)"""
-    _refuse(q.dtype == _BF16 and q.dim() in (2, 3), f"{name}: q is bfloat16 [rows, heads, head_dim] or [rows, heads * head_dim]")
-    if q.dim() == 3:
-        _refuse(q.shape[1] * q.shape[2] == width and (q.stride(2) == 1 or q.shape[2] == 1) and (q.stride(1) == q.shape[2] or q.shape[1] == 1),
-                f"{name}: q of shape {tuple(q.shape)} with strides {q.stride()}")
-    else:
-        _refuse(q.shape[1] == width and q.stride(1) == 1, f"{name}: q of shape {tuple(q.shape)} with strides {q.stride()}")
-    stride = q.stride(0) if q.shape[0] > 1 else width
-    _refuse(q.numel() == 0 or (q.data_ptr() % 16 == 0 and stride % 8 == 0), f"{name}: rows of q start on 16 bytes")
-    return q.shape[0], stride
+def _per_sequence(name: str, n: int, *vectors: torch.Tensor) -> None:
+    for t in vectors:
+        if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+            _refuse(name, f"lengths and slots are contiguous int32, {n} of them here")
 
 
-def _mass_workspace(name: str, workspace, need: int, device):
+def _state_of(name: str, state, dtype, n_kv_heads: int):
+    """mass or origin -> (rows, slots)"""
+    if state.dim() != 3 or state.dtype is not dtype or not state.is_contiguous() or state.shape[1] != n_kv_heads:
+        _refuse(name, f"state rows are contiguous {dtype} [rows, {n_kv_heads}, slots]")
+    return state.shape[0], state.shape[2]
+
+
+def _query_rows(name: str, q, n_q_heads: int, n_kv_heads: int, D: int):
+    """q [rows, heads, head_dim] or [rows, heads * head_dim] -> (rows, elements between them)"""
+    if n_q_heads <= 0 or n_q_heads % n_kv_heads != 0 or n_q_heads > 16 * n_kv_heads:
+        _refuse(name, f"{n_q_heads} query heads on {n_kv_heads} kv heads (up to 16 each)")
+    shape, strides = q.shape, q.stride()
+    if q.dtype is not _BF16 or (len(shape) == 3 and (shape[1:] != (n_q_heads, D) or strides[2] != 1 or (strides[1] != D and n_q_heads > 1))) or \
+            (len(shape) == 2 and (shape[1] != n_q_heads * D or strides[1] != 1)) or len(shape) not in (2, 3):
+        _refuse(name, f"q of {q.dtype} {tuple(shape)} with strides {strides}: bfloat16 rows of {n_q_heads} heads of {D}, side by side")
+    between = strides[0] if shape[0] > 1 else n_q_heads * D
+    if shape[0] and (q.data_ptr() % 16 or between % 8):
+        _refuse(name, "rows of q start on 16 bytes")
+    return shape[0], between
+
+
+def _mass_workspace(name: str, workspace, need: int, like) -> tuple[torch.Tensor, int]:
     if workspace is None:  # torch's allocator keeps it to the stream, or to the graph that is being captured
-        return torch.empty(need, dtype=torch.uint8, device=device)
-    _refuse(workspace.is_contiguous() and workspace.device == device and workspace.numel() * workspace.element_size() >= need,
-            f"{name}: a contiguous workspace of {need} bytes on {device}")
-    return workspace
+        return torch.empty(need, dtype=torch.uint8, device=like.device), need
+    size = workspace.numel() * workspace.element_size()
+    if size < need or not workspace.is_contiguous() or workspace.get_device() != like.get_device():
+        _refuse(name, f"a contiguous workspace of {need} bytes on {like.device}")
+    return workspace, size
 
 
 def paged_attn_decode_mass(q, k_cache, v_cache, block_tables, context_lens, mass, slots, n_q_heads: int, n_kv_heads: int,
@@ -312,22 +321,29 @@ def paged_attn_decode_mass(q, k_cache, v_cache, block_tables, context_lens, mass
     mass is set, so a row needs no clearing.  slots_out: rows that receive the result instead (slots: read only).
     Block ids outside the cache mask their tokens.  A graph captures it with its own workspace."""
     name = "paged_attn_decode_mass"
-    n, D, slots_out, width, stride = _mass_operands(name, (k_cache, v_cache), (block_tables,), context_lens, slots, slots_out, (mass,),
-                                                    n_kv_heads, block_size, (q,))
-    _refuse(n_q_heads > 0 and n_q_heads % n_kv_heads == 0 and n_q_heads // n_kv_heads <= 16,
-            f"{name}: {n_q_heads} query heads on {n_kv_heads} kv heads (up to 16 each)")
-    rows, q_stride = _rows_of(name, q, n_q_heads * D)
-    _refuse(rows == n, f"{name}: {rows} rows of q for {n} sequences")
+    if slots_out is None:
+        slots_out = slots
+    _here(name, q, k_cache, v_cache, block_tables, context_lens, mass, slots, slots_out)
+    n = context_lens.numel()
+    blocks, D = _cache_of(name, k_cache, n_kv_heads, block_size)
+    if _cache_of(name, v_cache, n_kv_heads, block_size) != (blocks, D):
+        _refuse(name, f"k_cache {tuple(k_cache.shape)}, v_cache {tuple(v_cache.shape)}")
+    width, between = _table_of(name, block_tables, n)
+    _per_sequence(name, n, context_lens, slots, slots_out)
+    rows, room = _state_of(name, mass, _F32, n_kv_heads)
+    n_rows, q_stride = _query_rows(name, q, n_q_heads, n_kv_heads, D)
+    if n_rows != n:
+        _refuse(name, f"{n_rows} rows of q for {n} sequences")
     if out is None:
         out = torch.empty((n, n_q_heads * D), dtype=_BF16, device=q.device)
-    _refuse(out.dtype == _BF16 and out.is_contiguous() and out.numel() == n * n_q_heads * D and out.device == q.device,
-            f"{name}: out is contiguous bfloat16 [{n}, {n_q_heads * D}]")
+    elif out.dtype is not _BF16 or not out.is_contiguous() or out.numel() != n * n_q_heads * D or out.get_device() != q.get_device():
+        _refuse(name, f"out is contiguous bfloat16 [{n}, {n_q_heads * D}]")
     if n == 0:
         return out
-    ws = _mass_workspace(name, workspace, lib.mi_paged_attn_decode_mass_workspace(n, n_q_heads, n_kv_heads, D, block_size, width), q.device)
-    check(lib.mi_paged_attn_decode_mass(ptr(q), q_stride, ptr(k_cache), ptr(v_cache), k_cache.shape[0], ptr(block_tables), stride, width,
-                                        ptr(context_lens), ptr(mass), mass.shape[0], mass.shape[2], ptr(slots), ptr(slots_out), ptr(out), ptr(ws),
-                                        ws.numel() * ws.element_size(), n, n_q_heads, n_kv_heads, D, block_size, float(scale), stream()), name)
+    ws, size = _mass_workspace(name, workspace, lib.mi_paged_attn_decode_mass_workspace(n, n_q_heads, n_kv_heads, D, block_size, width), q)
+    check(lib.mi_paged_attn_decode_mass(q.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(), blocks, block_tables.data_ptr(), between, width,
+                                        context_lens.data_ptr(), mass.data_ptr(), rows, room, slots.data_ptr(), slots_out.data_ptr(),
+                                        out.data_ptr(), ws.data_ptr(), size, n, n_q_heads, n_kv_heads, D, block_size, scale, stream()), name)
     return out
 
 
@@ -337,23 +353,27 @@ def prompt_attn_mass(q, k_cache, block_tables, cu_seqlens_q, kv_lens, max_seqlen
     sequence's rows, or its last `window`.  Tokens that the step stored have their mass set, those cached before are added to: portions
     of a prompt follow one another, and decode steps follow them."""
     name = "prompt_attn_mass"
-    n, D, slots_out, width, stride = _mass_operands(name, (k_cache,), (block_tables,), kv_lens, slots, slots_out, (mass,), n_kv_heads,
-                                                    block_size, (q, cu_seqlens_q))
-    _refuse(n_q_heads > 0 and n_q_heads % n_kv_heads == 0 and n_q_heads // n_kv_heads <= 16,
-            f"{name}: {n_q_heads} query heads on {n_kv_heads} kv heads (up to 16 each)")
-    rows, q_stride = _rows_of(name, q, n_q_heads * D)
-    _refuse(cu_seqlens_q.dtype == torch.int32 and cu_seqlens_q.is_contiguous() and cu_seqlens_q.numel() == n + 1,
-            f"{name}: cu_seqlens_q is contiguous int32, one more than the sequences")
-    _refuse(window >= 0 and max_seqlen_q >= 0, f"{name}: window {window}, max_seqlen_q {max_seqlen_q}")
+    if slots_out is None:
+        slots_out = slots
+    _here(name, q, k_cache, block_tables, cu_seqlens_q, kv_lens, mass, slots, slots_out)
+    n = kv_lens.numel()
+    blocks, D = _cache_of(name, k_cache, n_kv_heads, block_size)
+    width, between = _table_of(name, block_tables, n)
+    _per_sequence(name, n, kv_lens, slots, slots_out)
+    _per_sequence(name, n + 1, cu_seqlens_q)
+    rows, room = _state_of(name, mass, _F32, n_kv_heads)
+    n_rows, q_stride = _query_rows(name, q, n_q_heads, n_kv_heads, D)
+    if window < 0 or max_seqlen_q < 0:
+        _refuse(name, f"window {window}, max_seqlen_q {max_seqlen_q}")
     if n == 0:
         return
-    max_seqlen_q = min(int(max_seqlen_q), rows)
-    ws = _mass_workspace(name, workspace, lib.mi_prompt_attn_mass_workspace(n, rows, max(max_seqlen_q, 1), int(window), n_q_heads, n_kv_heads, D,
-                                                                            block_size, width), q.device)
-    check(lib.mi_prompt_attn_mass(ptr(q) if rows else ptr(k_cache), q_stride, rows, ptr(k_cache), k_cache.shape[0], ptr(block_tables), stride, width,
-                                  ptr(cu_seqlens_q), ptr(kv_lens), n, max_seqlen_q, int(window), ptr(mass), mass.shape[0], mass.shape[2],
-                                  ptr(slots), ptr(slots_out), ptr(ws), ws.numel() * ws.element_size(), n_q_heads, n_kv_heads, D, block_size,
-                                  float(scale), stream()), name)
+    most = min(max_seqlen_q, n_rows)
+    ws, size = _mass_workspace(name, workspace, lib.mi_prompt_attn_mass_workspace(n, n_rows, most, window, n_q_heads, n_kv_heads, D, block_size, width),
+                               q)
+    check(lib.mi_prompt_attn_mass(q.data_ptr() or ws.data_ptr(), q_stride, n_rows, k_cache.data_ptr(), blocks, block_tables.data_ptr(), between, width,
+                                  cu_seqlens_q.data_ptr(), kv_lens.data_ptr(), n, most, window, mass.data_ptr(), rows, room,
+                                  slots.data_ptr(), slots_out.data_ptr(), ws.data_ptr(), size, n_q_heads, n_kv_heads, D, block_size, scale,
+                                  stream()), name)
 
 
 def kv_cache_evict(k_cache, v_cache, block_tables, context_lens, mass, origin, evicted, slots, keep: int, sinks: int, recent: int,
@@ -367,27 +387,37 @@ def kv_cache_evict(k_cache, v_cache, block_tables, context_lens, mass, origin, e
     block_tables_out, which then receives what is kept.  slots_out likewise for the state's rows.  Head geometries of the plain cache layout
     (attention_is_plain) are not served."""
     name = "kv_cache_evict"
-    n_kv_heads = k_cache.shape[1] if k_cache.dim() == 4 else 0
-    tables = (block_tables,) if block_tables_out is None else (block_tables, block_tables_out)
+    if slots_out is None:
+        slots_out = slots
     if context_lens_out is None:
         context_lens_out = torch.empty_like(context_lens)
-    n, D, slots_out, width, stride = _mass_operands(name, (k_cache, v_cache), tables, context_lens, slots, slots_out, (mass, origin),
-                                                    n_kv_heads, block_size, (evicted, context_lens_out))
-    _refuse(origin.dtype == torch.int32, f"{name}: origin is int32")
-    _refuse(evicted.dtype == torch.int32 and evicted.is_contiguous() and evicted.shape == (mass.shape[0], 2),
-            f"{name}: evicted is contiguous int32 [{mass.shape[0]}, 2]")
-    _refuse(context_lens_out.dtype == torch.int32 and context_lens_out.is_contiguous() and context_lens_out.shape == context_lens.shape,
-            f"{name}: context_lens_out is contiguous int32 [{n}]")
-    _refuse(keep > 0 and sinks >= 0 and recent >= 0 and sinks + recent <= keep,
-            f"{name}: {sinks} first and {recent} newest tokens of {keep} kept")
-    _refuse(tables[-1].shape[1] >= -(-min(keep, width * block_size) // block_size), f"{name}: block_tables_out has no room for {keep} tokens")
+    if block_tables_out is None:
+        block_tables_out = block_tables
+    _here(name, k_cache, v_cache, block_tables, block_tables_out, context_lens, context_lens_out, mass, origin, evicted, slots, slots_out)
+    n = context_lens.numel()
+    n_kv_heads = k_cache.shape[1] if k_cache.dim() == 4 else 0
+    blocks, D = _cache_of(name, k_cache, n_kv_heads, block_size)
+    if _cache_of(name, v_cache, n_kv_heads, block_size) != (blocks, D):
+        _refuse(name, f"k_cache {tuple(k_cache.shape)}, v_cache {tuple(v_cache.shape)}")
+    width, between = _table_of(name, block_tables, n)
+    out_width, out_between = (width, between) if block_tables_out is block_tables else _table_of(name, block_tables_out, n)
+    _per_sequence(name, n, context_lens, context_lens_out, slots, slots_out)
+    rows, room = _state_of(name, mass, _F32, n_kv_heads)
+    if _state_of(name, origin, torch.int32, n_kv_heads) != (rows, room):
+        _refuse(name, f"mass {tuple(mass.shape)}, origin {tuple(origin.shape)}")
+    if evicted.dtype is not torch.int32 or evicted.shape != (rows, 2) or not evicted.is_contiguous():
+        _refuse(name, f"evicted is contiguous int32 [{rows}, 2]")
+    if keep <= 0 or sinks < 0 or recent < 0 or sinks + recent > keep:
+        _refuse(name, f"{sinks} first and {recent} newest tokens of {keep} kept")
+    if out_width * block_size < min(keep, width * block_size):
+        _refuse(name, f"block_tables_out has no room for {keep} tokens")
     if n == 0:
         return context_lens_out
-    ws = _mass_workspace(name, workspace, lib.mi_kv_cache_evict_workspace(n, n_kv_heads, int(keep), block_size, width), k_cache.device)
-    check(lib.mi_kv_cache_evict(ptr(k_cache), ptr(v_cache), k_cache.shape[0], ptr(block_tables), stride, ptr(tables[-1]),
-                                _table_stride(tables[-1]), width, ptr(context_lens), ptr(context_lens_out), ptr(mass), ptr(origin), ptr(evicted),
-                                mass.shape[0], mass.shape[2], ptr(slots), ptr(slots_out), int(keep), int(sinks), int(recent), ptr(ws),
-                                ws.numel() * ws.element_size(), n, n_kv_heads, D, block_size, stream()), name)
+    ws, size = _mass_workspace(name, workspace, lib.mi_kv_cache_evict_workspace(n, n_kv_heads, keep, block_size, width), k_cache)
+    check(lib.mi_kv_cache_evict(k_cache.data_ptr(), v_cache.data_ptr(), blocks, block_tables.data_ptr(), between, block_tables_out.data_ptr(),
+                                out_between, width, context_lens.data_ptr(), context_lens_out.data_ptr(), mass.data_ptr(), origin.data_ptr(),
+                                evicted.data_ptr(), rows, room, slots.data_ptr(), slots_out.data_ptr(), keep, sinks, recent,
+                                ws.data_ptr(), size, n, n_kv_heads, D, block_size, stream()), name)
     return context_lens_out
 
 

@@ -120,7 +120,7 @@ WRONG = [
 @pytest.mark.parametrize("case", range(len(WRONG)))
 def test_wrappers_refuse(monkeypatch, case):
     """the wrappers' own checks (the device's aside), each alone wrong"""
-    monkeypatch.setattr(ops, "_on_current_device", lambda *a: None)
+    monkeypatch.setattr(ops, "_here", lambda *a: 0)
     which, key, change = WRONG[case]
     for w in which.split():
         a = good()
