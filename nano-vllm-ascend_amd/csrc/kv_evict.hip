@@ -29,8 +29,8 @@ struct Evict {
   int64_t rows, len;
   const int32_t *slots, *slots_out;
   int keep, sinks, recent;
-  int32_t *head;               // [batch][n_kv][2]: what the second launch does, tokens
-  int32_t *src, *free, *moved; // [batch][n_kv][keep]
+  int32_t* head;                // [batch][n_kv][2]: what the second launch does, tokens
+  int32_t *src, *free, *moved;  // [batch][n_kv][keep]: where each place's token was; places that became free, slots that move there
 };
 
 enum { NOTHING = -1, SAME_PLACES = 0, LISTED = 1 };
@@ -48,25 +48,164 @@ struct Tokens {
   const int32_t* origin;
   int kept, dropped, ctx, sinks, recent;
   __device__ int position(int j) const { return j < kept ? origin[j] : j + dropped; }
-  __device__ uint32_t key(int j) const {
-    const int p = position(j);
-    return p < sinks || p >= ctx + dropped - recent ? ~0u : key_of(mass[j]);
-  }
+  __device__ uint32_t key_at(int position, float m) const { return position < sinks || position >= ctx + dropped - recent ? ~0u : key_of(m); }
+  __device__ uint32_t key(int j) const { return key_at(position(j), mass[j]); }
 };
 
-// One workgroup per (kv head, sequence): the keep-th largest key by four passes of 8 bits over the keys (counts in LDS, a column of its
-// own per lane: masses share their leading bits, and lanes that add to one address wait for one another), then the lists in slot order.
-constexpr int CT = 1024, CW = CT / 64;
+// One workgroup per (kv head, sequence): the keep-th largest key digit by digit (11, 11 and 10 bits, counts in LDS), then the lists in slot
+// order.  A wave has a contiguous part of the slots, 64 at a time, so that ranks need the waves' totals and ballots only.  Up to HELD tokens the
+// keys are kept in LDS; longer contexts are read again in each of the six walks.  Masses share their leading bits, and lanes that add to one address
+// wait for one another: two copies of the counts.
+constexpr int CT = 1024, CW = CT / 64, BINS = 2048, COPIES = 2;
 
+struct Counts {
+  uint32_t count[BINS * COPIES];
+  uint32_t in_wave[CW], found[3];
+  int equal[CW], n_free[CW], n_moved[CW];
+};
+
+template <bool IN_LDS>
+__device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts& sm, uint32_t* held, float* mass_out, int32_t* origin_out, bool same_row,
+                                       int64_t unit) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int part = ((tk.ctx + CT - 1) / CT) * 64, j0 = min(wave * part, tk.ctx), j1 = min(j0 + part, tk.ctx);
+  auto key = [&](int j) { return IN_LDS ? held[j] : tk.key(j); };
+  // f(slot, key, the slot is there) for the wave's part; four keys are on their way at a time
+  auto walk = [&](auto&& f) __attribute__((always_inline)) {
+    for (int j = j0 + lane; j - lane < j1; j += 256) {
+      uint32_t k[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) k[i] = j + 64 * i < j1 ? key(j + 64 * i) : 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (j - lane + 64 * i < j1) f(j + 64 * i, k[i], j + 64 * i < j1);
+    }
+  };
+  if (IN_LDS) {
+    for (int j = tid; j < tk.ctx; j += 8 * CT) {
+      float m[8];
+      int p[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = min(j + CT * i, tk.ctx - 1);
+        m[i] = tk.mass[at];
+        p[i] = tk.kept > 0 ? tk.origin[min(at, tk.kept - 1)] : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = j + CT * i;
+        if (at < tk.ctx) held[at] = tk.key_at(at < tk.kept ? p[i] : at + tk.dropped, m[i]);
+      }
+    }
+  }
+  uint32_t prefix = 0, need = a.keep;
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    *reinterpret_cast<uint4*>(&sm.count[4 * tid]) = uint4{0u, 0u, 0u, 0u};
+    __syncthreads();
+    walk([&](int, uint32_t k, bool on) {
+      if (on && (pass == 0 || k >> (shift + bits) == prefix)) atomicAdd(&sm.count[(k >> shift & ((1u << bits) - 1)) * COPIES + (lane & (COPIES - 1))], 1u);
+    });
+    __syncthreads();
+    // thread t: bins 2047 - 2 t and the one below, from the top
+    const uint4 v = *reinterpret_cast<const uint4*>(&sm.count[(BINS - 2 - 2 * tid) * COPIES]);
+    const uint32_t c[2] = {v.z + v.w, v.x + v.y};
+    uint32_t upto = c[0] + c[1];
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t o = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += o;
+    }
+    if (lane == 63) sm.in_wave[wave] = upto;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) upto += sm.in_wave[w];
+    uint32_t before = upto - c[0] - c[1];
+    if (before < need && need <= upto) {
+      const int i = before + c[0] < need;
+      if (i) before += c[0];
+      sm.found[0] = prefix << bits | (uint32_t)(BINS - 1 - 2 * tid - i);
+      sm.found[1] = need - before;
+      sm.found[2] = c[i];
+    }
+    __syncthreads();
+    prefix = sm.found[0], need = sm.found[1];
+  }
+  // kept: keys above `prefix`, and the first `need` of those that are equal to it
+  const bool all_equal = sm.found[2] == need;  // every one of those (the usual case: one): no ranks among them
+  int ties = 0;
+  if (!all_equal) {
+    int n_equal = 0;
+    walk([&](int, uint32_t k, bool on) { n_equal += __popcll(__ballot(on && k == prefix)); });
+    if (lane == 0) sm.equal[wave] = n_equal;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) ties += sm.equal[w];
+  }
+  const uint64_t below = (1ull << lane) - 1;
+  // (the ballots of a chunk; `tie`: equal keys before it)
+  auto stays = [&](uint32_t k, bool on, int& tie) {
+    if (all_equal) return on && k >= prefix;
+    const uint64_t same = __ballot(on && k == prefix);
+    const bool yes = on && (k > prefix || (k == prefix && tie + __popcll(same & below) < (int)need));
+    tie += __popcll(same);
+    return yes;
+  };
+  int frees = 0, moves = 0, tie = ties;
+  walk([&](int j, uint32_t k, bool on) {
+    const bool kept = stays(k, on, tie);
+    frees += __popcll(__ballot(on && j < a.keep && !kept));
+    moves += __popcll(__ballot(j >= a.keep && kept));
+  });
+  if (lane == 0) sm.n_free[wave] = frees, sm.n_moved[wave] = moves;
+  __syncthreads();
+  int at_free = 0, at_moved = 0, all = 0;
+  for (int w = 0; w < CW; ++w) {
+    if (w < wave) at_free += sm.n_free[w], at_moved += sm.n_moved[w];
+    all += sm.n_free[w];
+  }
+  int32_t* const free = a.free + unit * a.keep;
+  int32_t* const moved = a.moved + unit * a.keep;
+  int32_t* const src = a.src + unit * a.keep;
+  tie = ties;
+  walk([&](int j, uint32_t k, bool on) {
+    const bool kept = stays(k, on, tie), gone = on && j < a.keep && !kept, goes = j >= a.keep && kept;
+    const uint64_t all_gone = __ballot(gone), all_go = __ballot(goes);
+    if (gone) free[at_free + __popcll(all_gone & below)] = j;
+    if (goes) moved[at_moved + __popcll(all_go & below)] = j;
+    at_free += __popcll(all_gone);
+    at_moved += __popcll(all_go);
+    if (kept && j < a.keep) src[j] = j;
+  });
+  __threadfence_block();
+  __syncthreads();
+  for (int i = tid; i < all; i += CT) src[free[i]] = moved[i];
+  __threadfence_block();
+  __syncthreads();
+  // what a place's mass and position are now: in place those of moved tokens, and positions that were not written down yet
+  for (int j = tid; j < a.keep; j += 4 * CT) {
+    int from[4], p[4];
+    float m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) from[i] = src[min(j + CT * i, a.keep - 1)];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = tk.mass[from[i]], p[i] = tk.position(from[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int to = j + CT * i;
+      if (to >= a.keep || (same_row && from[i] == to && to < tk.kept)) continue;
+      if (!same_row || from[i] != to) mass_out[to] = m[i];
+      origin_out[to] = p[i];
+    }
+  }
+}
+
+template <int HELD>
 __global__ __launch_bounds__(CT) void evict_choose_kernel(Evict a) {
-  __shared__ uint32_t count[256 * 32];
-  __shared__ uint32_t total[256];
-  __shared__ uint32_t sm_prefix, sm_need;
-  __shared__ int sm_more[2 * CW], sm_equal[2 * CW];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ __attribute__((aligned(16))) Counts sm;
+  __shared__ uint32_t held[HELD];
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const int ctx = max(a.lens[b], 0);
-  const int64_t r = a.slots[b], ro = a.slots_out[b];
-  int32_t* head = a.head + ((int64_t)b * a.n_kv + h) * 2;
+  const int64_t r = a.slots[b], ro = a.slots_out[b], unit = (int64_t)b * a.n_kv + h;
+  int32_t* head = a.head + unit * 2;
   // (a context that has outgrown its pages or its row stays as it is)
   const bool valid = r >= 0 && r < a.rows && ro >= 0 && ro < a.rows && ctx <= a.cap && ctx <= a.len;
   if (tid == 0) {
@@ -87,142 +226,47 @@ __global__ __launch_bounds__(CT) void evict_choose_kernel(Evict a) {
     }
     return;
   }
-
-  uint32_t prefix = 0, need = a.keep;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256 * 32; i += CT) count[i] = 0;
-    __syncthreads();
-    for (int j = tid; j < ctx; j += CT) {
-      const uint32_t k = tk.key(j);
-      if (shift == 24 || k >> (shift + 8) == prefix) atomicAdd(&count[((k >> shift) & 255) * 32 + (lane & 31)], 1u);
-    }
-    __syncthreads();
-    if (tid < 256) {
-      uint32_t n = 0;
-      for (int i = 0; i < 32; ++i) n += count[tid * 32 + ((i + tid) & 31)];
-      total[tid] = n;
-    }
-    __syncthreads();
-    if (wave == 0) {  // lane i: bins 255 - 4 i downwards; the one in which the need-th largest is
-      uint32_t c[4], sum = 0;
-      for (int i = 0; i < 4; ++i) sum += c[i] = total[255 - 4 * lane - i];
-      uint32_t upto = sum;
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(upto, d, 64);
-        if (lane >= d) upto += o;
-      }
-      uint32_t before = upto - sum;
-      if (before < need && need <= upto) {
-        int i = 0;
-        while (before + c[i] < need) before += c[i++];
-        sm_prefix = prefix << 8 | (uint32_t)(255 - 4 * lane - i);
-        sm_need = need - before;
-      }
-    }
-    __syncthreads();
-    prefix = sm_prefix, need = sm_need;
-  }
-  // kept: keys above `prefix`, and of those equal to it the first `need`.  Wave w counts its part of the slots below keep and its part of
-  // those behind, in slot order.
-  const int part_lo = ((a.keep + CT - 1) / CT) * 64, part_hi = ((ctx - a.keep + CT - 1) / CT) * 64;
-  auto range = [&](int side, int& j0, int& j1) {
-    j0 = side ? min(a.keep + wave * part_hi, ctx) : min(wave * part_lo, a.keep);
-    j1 = side ? min(j0 + part_hi, ctx) : min(j0 + part_lo, a.keep);
-  };
-  for (int side = 0; side < 2; ++side) {
-    int j0, j1, more = 0, equal = 0;
-    range(side, j0, j1);
-    for (int j = j0; j < j1; j += 64) {
-      const bool on = j + lane < j1;
-      const uint32_t k = on ? tk.key(j + lane) : 0;
-      more += __popcll(__ballot(on && k > prefix));
-      equal += __popcll(__ballot(on && k == prefix));
-    }
-    if (lane == 0) sm_more[side * CW + wave] = more, sm_equal[side * CW + wave] = equal;
-  }
-  __syncthreads();
-  int32_t* src = a.src + ((int64_t)b * a.n_kv + h) * a.keep;
-  int32_t* free = a.free + ((int64_t)b * a.n_kv + h) * a.keep;
-  int32_t* moved = a.moved + ((int64_t)b * a.n_kv + h) * a.keep;
-  const uint64_t below = (1ull << lane) - 1;
-  int n_free = 0;
-  for (int side = 0; side < 2; ++side) {
-    int j0, j1, equal = 0, listed = 0;
-    range(side, j0, j1);
-    for (int p = 0; p < side * CW + wave; ++p) {
-      const int taken = max(0, min(sm_equal[p], (int)need - equal)) + sm_more[p];
-      equal += sm_equal[p];
-      const int at = p < CW ? min(p * part_lo, a.keep) : 0;
-      if (p >= CW) listed += taken;
-      else if (side == 0) listed += min(at + part_lo, a.keep) - at - taken;
-    }
-    for (int j = j0; j < j1; j += 64) {
-      const bool on = j + lane < j1;
-      const uint32_t k = on ? tk.key(j + lane) : 0;
-      const uint64_t ties = __ballot(on && k == prefix);
-      const bool stays = on && (k > prefix || (k == prefix && equal + __popcll(ties & below) < (int)need));
-      const bool list = on && (side ? stays : !stays);
-      const uint64_t lists = __ballot(list);
-      if (side == 0 && on) src[j + lane] = j + lane;
-      if (list) (side ? moved : free)[listed + __popcll(lists & below)] = j + lane;
-      equal += __popcll(ties);
-      listed += __popcll(lists);
-    }
-    if (side == 0) n_free = listed;
-  }
-  // all waves' lists, and their number: the last wave of the first side ends with it
-  __syncthreads();
-  if (wave == CW - 1 && lane == 0) sm_need = (uint32_t)n_free;
-  __threadfence_block();
-  __syncthreads();
-  n_free = (int)sm_need;
-  for (int i = tid; i < n_free; i += CT) {
-    const int to = free[i], from = moved[i];
-    src[to] = from;
-    if (r == ro) {
-      mass_out[to] = tk.mass[from];
-      origin_out[to] = tk.position(from);
-    }
-  }
-  __threadfence_block();
-  __syncthreads();
-  // the positions of slots at or behind what an earlier eviction left are written down now
-  for (int j = tid; j < a.keep; j += CT) {
-    const int from = src[j];
-    if (r != ro) {
-      mass_out[j] = tk.mass[from];
-      origin_out[j] = tk.position(from);
-    } else if (from == j && j >= tk.kept) {
-      origin_out[j] = j + tk.dropped;
-    }
-  }
+  if (ctx <= HELD) choose<true>(a, tk, sm, held, mass_out, origin_out, r == ro, unit);
+  else choose<false>(a, tk, sm, held, mass_out, origin_out, r == ro, unit);
 }
 
-// A wave: one tile of 16 places of one kv head.  K goes in the 16-byte pieces that a token is in; a piece of V holds four tokens, so that a
-// wave builds whole pieces of its tile from those of the tokens that move there and what is there already.
+// lengths and rows, once everything has read the ones before
+__device__ __forceinline__ void finish(const Evict& a, int b, int mode, int ctx, int n) {
+  a.lens_out[b] = mode == NOTHING ? ctx : n;
+  if (mode == NOTHING) return;
+  const int64_t r = a.slots[b], ro = a.slots_out[b];
+  const int kept = a.evicted[2 * r], dropped = a.evicted[2 * r + 1];
+  a.evicted[2 * ro] = mode == LISTED ? n : kept;
+  a.evicted[2 * ro + 1] = mode == LISTED ? dropped + ctx - n : dropped;
+}
+
+// the two 16-bit values of token f % 4 of a 16-byte piece of V (dims d and d + 16) in place of those of token e of v
+__device__ __forceinline__ void patch(u32x4& v, int e, const u32x4& x, int f) {
+  const uint32_t lo = (f & 2 ? x[1] : x[0]) >> (f & 1) * 16 & 0xffffu, hi = (f & 2 ? x[3] : x[2]) >> (f & 1) * 16 & 0xffffu;
+  const uint32_t sh = (e & 1) * 16, field = 0xffffu << sh;
+  v[e >> 1] = (v[e >> 1] & ~field) | lo << sh;
+  v[2 + (e >> 1)] = (v[2 + (e >> 1)] & ~field) | hi << sh;
+}
+
+// A wave: one tile of 16 places of one kv head; places whose page and slot are the old ones are left.  K goes in the 16-byte pieces that a token is
+// in; a piece of V holds four tokens, so that a wave builds whole pieces of its tile from those of the tokens that move there and what is there
+// already.  A token's K is in D / 8 lines of the cache and its V in a quarter of a tile: what bounds this is the lines that hold a mover, not
+// the movers' bytes.  (Teams of 16 lanes with four places each, taken from the list of movers, touch the same lines: 39 us against 42 for 32
+// sequences back to 4096 tokens, 171 against 167 for 8 from 32768, and 12 against 4 for one from 1100 to 1024.)
 template <int DB>
 __global__ __launch_bounds__(256) void evict_move_kernel(Evict a) {
   constexpr int TILE = 512 * DB;
   const int h = blockIdx.x, b = blockIdx.z, lane = threadIdx.x & 63, t = blockIdx.y * 4 + (threadIdx.x >> 6);
-  const int32_t* head = a.head + ((int64_t)b * a.n_kv + h) * 2;
-  const int mode = head[0], ctx = head[1], n = min(ctx, a.keep);
-  if (h == 0 && t == 0 && lane == 0) {
-    a.lens_out[b] = mode == NOTHING ? ctx : n;
-    if (mode != NOTHING) {
-      const int64_t r = a.slots[b], ro = a.slots_out[b];
-      const int kept = a.evicted[2 * r], dropped = a.evicted[2 * r + 1];
-      a.evicted[2 * ro] = mode == LISTED ? n : kept;
-      a.evicted[2 * ro + 1] = mode == LISTED ? dropped + ctx - n : dropped;
-    }
-  }
+  const int64_t unit = (int64_t)b * a.n_kv + h;
+  const int mode = a.head[unit * 2], ctx = a.head[unit * 2 + 1], n = min(ctx, a.keep);
+  if (h == 0 && t == 0 && lane == 0) finish(a, b, mode, ctx, n);
   if (mode == NOTHING || 16 * t >= n) return;
   const int g = lane >> 4, c = lane & 15;
   const int32_t *row = a.table + (int64_t)b * a.table_stride, *row_out = a.table_out + (int64_t)b * a.table_out_stride;
   const int to = row_out[t / a.tpb];
   const int slot = 16 * t + c;
-  const int from = slot < n ? (mode == LISTED ? a.src[((int64_t)b * a.n_kv + h) * a.keep + slot] : slot) : slot;
+  const int from = slot < n && mode == LISTED ? a.src[unit * a.keep + slot] : slot;
   const int page = slot < n ? row[from / (16 * a.tpb)] : -1;
-  // a page that names no block of the cache is neither read nor written
   const bool moves = slot < n && page >= 0 && page < a.num_blocks && (from != slot || page != to);
   if (to < 0 || to >= a.num_blocks || !__any(moves)) return;
   const int64_t dst = (((int64_t)to * a.n_kv + h) * a.tpb + t % a.tpb) * TILE;
@@ -235,32 +279,30 @@ __global__ __launch_bounds__(256) void evict_move_kernel(Evict a) {
 #pragma unroll
     for (int kk = 0; kk < DB; ++kk) *reinterpret_cast<u32x4*>(a.kc + dst + kk * 512 + (g * 16 + c) * 8) = x[kk];
   }
-  u32x4 v[DB];
-#pragma unroll
-  for (int kk = 0; kk < DB; ++kk) v[kk] = *reinterpret_cast<const u32x4*>(a.vc + dst + kk * 512 + lane * 8);
-  bool any = false;
+  u32x4 v[DB], y[4][DB];
+  int f[4];
+  bool mv[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {  // token 4 g + e of the tile
     const int who = 4 * g + e;
-    const bool mv = __shfl((int)moves, who, 64);
-    const int f = __shfl(from, who, 64);
+    mv[e] = __shfl((int)moves, who, 64);
+    f[e] = __shfl(from, who, 64);
     const int64_t s = ((int64_t)__shfl((int)(src >> 32), who, 64) << 32) | (uint32_t)__shfl((int)(uint32_t)src, who, 64);
-    if (mv) {
-      any = true;
-      const int fe = f % 4;
+    if (mv[e])
 #pragma unroll
-      for (int kk = 0; kk < DB; ++kk) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(a.vc + s + kk * 512 + (f % 16 / 4 * 16 + c) * 8);
-        const uint32_t lo = (fe >= 2 ? x[1] : x[0]) >> (fe & 1) * 16 & 0xffffu, hi = (fe >= 2 ? x[3] : x[2]) >> (fe & 1) * 16 & 0xffffu;
-        const uint32_t sh = (e & 1) * 16, field = 0xffffu << sh;
-        v[kk][e >> 1] = (v[kk][e >> 1] & ~field) | lo << sh;
-        v[kk][2 + (e >> 1)] = (v[kk][2 + (e >> 1)] & ~field) | hi << sh;
-      }
-    }
+      for (int kk = 0; kk < DB; ++kk) y[e][kk] = *reinterpret_cast<const u32x4*>(a.vc + s + kk * 512 + (f[e] % 16 / 4 * 16 + c) * 8);
   }
-  if (any)
+  if (!(mv[0] || mv[1] || mv[2] || mv[3])) return;
+  if (!(mv[0] && mv[1] && mv[2] && mv[3]))
 #pragma unroll
-    for (int kk = 0; kk < DB; ++kk) *reinterpret_cast<u32x4*>(a.vc + dst + kk * 512 + lane * 8) = v[kk];
+    for (int kk = 0; kk < DB; ++kk) v[kk] = *reinterpret_cast<const u32x4*>(a.vc + dst + kk * 512 + lane * 8);
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (mv[e])
+#pragma unroll
+      for (int kk = 0; kk < DB; ++kk) patch(v[kk], e, y[e][kk], f[e]);
+#pragma unroll
+  for (int kk = 0; kk < DB; ++kk) *reinterpret_cast<u32x4*>(a.vc + dst + kk * 512 + lane * 8) = v[kk];
 }
 
 size_t evict_ints(int64_t batch, int64_t n_kv, int64_t keep, int64_t cap) { return batch * n_kv * (2 + (keep < cap ? 3 * keep : 0)); }
@@ -307,8 +349,9 @@ extern "C" int mi_kv_cache_evict(mi_bf16* k_cache, mi_bf16* v_cache, int64_t num
   a.slots = slots, a.slots_out = slots_out, a.keep = keep, a.sinks = sinks, a.recent = recent;
   a.head = static_cast<int32_t*>(workspace);
   a.src = a.head + units * 2, a.free = a.src + units * keep, a.moved = a.free + units * keep;
-  evict_choose_kernel<<<dim3(n_kv_heads, batch), CT, 0, S(stream)>>>(a);
-  const dim3 grid(n_kv_heads, (unsigned)blocks, batch);
+  const dim3 units_grid(n_kv_heads, batch), grid(n_kv_heads, (unsigned)blocks, batch);
+  if (cap <= 8192) evict_choose_kernel<8192><<<units_grid, CT, 0, S(stream)>>>(a);
+  else evict_choose_kernel<32768><<<units_grid, CT, 0, S(stream)>>>(a);
   if (head_dim == 128) evict_move_kernel<4><<<grid, 256, 0, S(stream)>>>(a);
   else evict_move_kernel<2><<<grid, 256, 0, S(stream)>>>(a);
   return check_launch();
