@@ -120,6 +120,8 @@ __global__ __launch_bounds__(DW * 64) void decode_mass_kernel(DecodeMass a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, n = lane & 15;
   const int32_t* row = a.pg.table + (int64_t)b * a.pg.table_stride;
+  const float* const had = a.rows.in(b, h);  // (read here: a dependent read less at the end)
+  float* const now = a.rows.out(b, h);
   const int c0 = deal(split * DW + wave), c1 = deal(split * DW + wave + 1);
 
   bf16x8 Q[DB];
@@ -283,31 +285,42 @@ __global__ __launch_bounds__(DW * 64) void decode_mass_kernel(DecodeMass a) {
   }
   if (a.splits > 1) return;
   __syncthreads();
-  const float* had = a.rows.in(b, h);
-  float* now = a.rows.out(b, h);
   if (now == nullptr) return;
   const int end = (int)min((int64_t)ctx, a.rows.len);
   for (int j = threadIdx.x; j < end; j += DW * 64) {
     float w = 0.f;
+#pragma unroll 4
     for (int hn = 0; hn < G; ++hn) w += __builtin_amdgcn_exp2f(a.scores[(row0 + hn) * a.pg.cap + j] - sm_M[hn]) * sm_inv[hn];
     now[j] = (j < ctx - 1 && had != nullptr ? had[j] : 0.f) + w;
   }
 }
 
-// joins the splits: grid (kv heads, shares of the context, batch), 4 waves
+// joins the splits: grid (kv heads, shares of the context, batch), 4 waves.  A few dependent reads long, so what does not depend on the sums - the
+// scores of a thread's first token, its mass so far - is asked for ahead of them.
 template <int D>
 __global__ __launch_bounds__(256) void decode_mass_join_kernel(DecodeMass a) {
   __shared__ float sm_M[16], sm_inv[16], sm_e[16][MAX_SPLITS];
-  const int h = blockIdx.x, b = blockIdx.z, G = a.G;
-  const int ctx = min(max(a.lens[b], 0), a.pg.cap);
+  const int h = blockIdx.x, b = blockIdx.z, G = a.G, lane = threadIdx.x & 63;
   const int64_t row0 = (int64_t)b * a.pg.n_kv * G + (int64_t)h * G;
-  const int lane = threadIdx.x & 63;
+  const int ctx = min(max(a.lens[b], 0), a.pg.cap), end = (int)min((int64_t)ctx, a.rows.len);
+  const float* const had = a.rows.in(b, h);
+  float* const now = a.rows.out(b, h);
+  const float* const scores = a.scores + row0 * a.pg.cap;
+  int j = blockIdx.y * 256 + threadIdx.x;
+  auto old = [&](int at) { return at < ctx - 1 && had != nullptr ? had[at] : 0.f; };
+  const bool first = now != nullptr && j < end;
+  float s[16], was = 0.f;
+  if (first) {
+#pragma unroll
+    for (int hn = 0; hn < 16; ++hn)
+      if (hn < G) s[hn] = scores[(int64_t)hn * a.pg.cap + j];
+    was = old(j);
+  }
   for (int hn = threadIdx.x >> 6; hn < G; hn += 4) {
     const bool on = lane < a.splits;
-    const float* ml = a.part_ml + ((row0 + hn) * a.splits + (on ? lane : 0)) * 2;
-    const float m = on ? ml[0] : -INFINITY, l = on ? ml[1] : 0.f;
-    const float M = wave_max(m), ms = M == -INFINITY ? 0.f : M;
-    const float e = __builtin_amdgcn_exp2f(m - ms), L = wave_sum(e * l);
+    const float2 ml = on ? *reinterpret_cast<const float2*>(a.part_ml + ((row0 + hn) * a.splits + lane) * 2) : float2{-INFINITY, 0.f};
+    const float M = wave_max(ml.x), ms = M == -INFINITY ? 0.f : M;
+    const float e = __builtin_amdgcn_exp2f(ml.x - ms), L = wave_sum(e * ml.y);
     sm_e[hn][lane] = e;
     if (lane == 0) {
       sm_M[hn] = ms;
@@ -315,23 +328,33 @@ __global__ __launch_bounds__(256) void decode_mass_join_kernel(DecodeMass a) {
     }
   }
   __syncthreads();
+  if (first) {
+    float w = 0.f;
+#pragma unroll
+    for (int hn = 0; hn < 16; ++hn)
+      if (hn < G) w += __builtin_amdgcn_exp2f(s[hn] - sm_M[hn]) * sm_inv[hn];
+    now[j] = was + w;
+    for (j += gridDim.y * 256; j < end; j += gridDim.y * 256) {
+      w = 0.f;
+#pragma unroll 8
+      for (int hn = 0; hn < G; ++hn) w += __builtin_amdgcn_exp2f(scores[(int64_t)hn * a.pg.cap + j] - sm_M[hn]) * sm_inv[hn];
+      now[j] = old(j) + w;
+    }
+  }
   for (int idx = blockIdx.y * 256 + threadIdx.x; idx < G * D; idx += gridDim.y * 256) {
     const int hn = idx / D, d = idx % D;
     float o = 0.f;
-    for (int s = 0; s < a.splits; ++s) {
-      const float e = sm_e[hn][s];
-      if (e != 0.f) o += e * a.part_o[((row0 + hn) * a.splits + s) * D + d];  // (an empty split wrote no sums)
+    for (int p = 0; p < a.splits; p += 8) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = a.part_o[((row0 + hn) * a.splits + min(p + i, a.splits - 1)) * D + d];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float e = p + i < a.splits ? sm_e[hn][p + i] : 0.f;
+        o += e != 0.f ? e * v[i] : 0.f;  // (an empty split wrote no sums)
+      }
     }
     a.out[(row0 + hn) * D + d] = f2bf(o * sm_inv[hn]);
-  }
-  const float* had = a.rows.in(b, h);
-  float* now = a.rows.out(b, h);
-  if (now == nullptr) return;
-  const int end = (int)min((int64_t)ctx, a.rows.len);
-  for (int j = blockIdx.y * 256 + threadIdx.x; j < end; j += gridDim.y * 256) {
-    float w = 0.f;
-    for (int hn = 0; hn < G; ++hn) w += __builtin_amdgcn_exp2f(a.scores[(row0 + hn) * a.pg.cap + j] - sm_M[hn]) * sm_inv[hn];
-    now[j] = (j < ctx - 1 && had != nullptr ? had[j] : 0.f) + w;
   }
 }
 
@@ -918,10 +941,13 @@ PromptPlan prompt_plan(int n_seqs, int64_t n_tokens, int max_seqlen_q, int windo
   return p;
 }
 
+// A workgroup fills a CU.  256 units and more are left whole (two halves each: 26 + 4 us against 25 for 32 sequences of 1024 tokens on 8 kv heads);
+// fewer are split into some four workgroups a CU, so that contexts of all lengths share the chip evenly (24 sequences of 101 to 8000 tokens on 4
+// kv heads: 55 us with one a CU, 48 with four), of 256 tokens at least.
 int decode_splits(int batch, int n_kv, int64_t cap) {
-  const int64_t units = (int64_t)batch * n_kv;
-  const int64_t by_chip = 256 / std::max<int64_t>(units, 1), by_length = (cap + 32 * DW - 1) / (32 * DW);
-  return (int)std::max<int64_t>(1, std::min<int64_t>({by_chip, by_length, MAX_SPLITS}));
+  const int64_t units = std::max<int64_t>((int64_t)batch * n_kv, 1);
+  if (units >= 256) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({1024 / units, (cap + 32 * DW - 1) / (32 * DW), MAX_SPLITS}));
 }
 
 size_t decode_bytes(int batch, int n_q, int D, int splits, int64_t cap) {
@@ -976,7 +1002,7 @@ extern "C" int mi_paged_attn_decode_mass(const mi_bf16* q, int64_t q_row_stride,
   if (head_dim == 128) decode_mass_kernel<4><<<grid, DW * 64, 0, S(stream)>>>(a);
   else decode_mass_kernel<2><<<grid, DW * 64, 0, S(stream)>>>(a);
   if (splits > 1) {
-    const int shares = (int)std::max<int64_t>(1, std::min<int64_t>((cap + 1023) / 1024, 2048 / ((int64_t)batch * n_kv_heads)));
+    const int shares = (int)std::max<int64_t>(1, std::min<int64_t>((cap + 255) / 256, 8192 / ((int64_t)batch * n_kv_heads)));
     const dim3 jg(n_kv_heads, shares, batch);
     if (head_dim == 128) decode_mass_join_kernel<128><<<jg, 256, 0, S(stream)>>>(a);
     else decode_mass_join_kernel<64><<<jg, 256, 0, S(stream)>>>(a);
