@@ -376,10 +376,9 @@ struct PromptMass {
   MassRows rows;
   uint16_t* packed;  // [n_kv][tiles][D * 32] rows in operand order
   float* part_ml;    // [n_kv][parts][tiles * 32][2]
-  float* part_sum;   // [n_kv][row_parts][n_seqs][cap]
   float* lse;        // [n_kv][tiles * 32]: log2 of the row's sum of exp2, infinity for a row that sees nothing
   int64_t tiles;     // 32-row tiles of a kv head, all sequences
-  int n_tokens, n_seqs, window, max_rows, G, parts, row_parts;
+  int n_tokens, window, max_rows, G, parts;
   float scale_log2e;
 };
 
@@ -406,44 +405,6 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptMass& a, int b) {
 
 // token of the 32 that register r of lane half `hf` holds
 __device__ __forceinline__ int key_of(int r, int hf) { return (r >> 2) * 8 + hf * 4 + (r & 3); }
-
-// A stream of 64-row pairs of tiles goes through three buffers in LDS, by way of registers: in step i pair i + 2 is written and pair i + 3
-// requested, so that the products of the next tile always run under the powers of this one.  (Copied to LDS without registers, a tile's reads wait
-// for every copy in flight: the compiler tells them apart by nothing but the array.)
-__device__ __forceinline__ void pair_done() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-__device__ __forceinline__ int after(int slot) { return slot == 2 ? 0 : slot + 1; }
-
-// One step: the products of the next tile (fragment j of the stream from LDS by two of the wave's own), and between the
-// matrix instructions, 32 cycles each and of two independent chains, what `power` does with score r of this tile's side t and `add` with what
-// came of it: 4 + 8 + 4 cycles for 32 scores, the time of the 16 (8) products.  A wave issues in order, so the order is written down here;
-// the compiler's own has the products of a chain behind one another, each waiting for the last.
-template <int J, typename Read, typename Multiply, typename Power, typename Add>
-__device__ __forceinline__ void multiply_among(Read&& read, Multiply&& multiply, Power&& power, Add&& add) {
-  constexpr int N = 32 / (2 * J);  // scores a matrix instruction
-  constexpr int AHEAD = 4;         // fragments on their way from LDS
-  u32x4 f[J];
-#pragma unroll
-  for (int j = 0; j < AHEAD; ++j) f[j] = read(j);
-  float e[N];
-  __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-  for (int i = 0; i < 2 * J; ++i) {
-    float was[N];
-#pragma unroll
-    for (int v = 0; v < N; ++v) was[v] = e[v];
-#pragma unroll
-    for (int v = 0; v < N; ++v) e[v] = power((i * N + v) >> 4, (i * N + v) & 15);
-#pragma unroll
-    for (int v = 0; v < N; ++v)
-      if (i > 0) add(((i - 1) * N + v) >> 4, ((i - 1) * N + v) & 15, was[v]);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(i & 1, i >> 1, f[i >> 1]);
-    if ((i & 1) && (i >> 1) + AHEAD < J) f[(i >> 1) + AHEAD] = read((i >> 1) + AHEAD);
-    __builtin_amdgcn_sched_barrier(0);
-  }
-#pragma unroll
-  for (int v = 0; v < N; ++v) add(((2 * J - 1) * N + v) >> 4, ((2 * J - 1) * N + v) & 15, e[v]);
-}
 
 // ---- the row sums: a wave's 64 rows, two tiles of 32
 template <int D>
@@ -520,7 +481,9 @@ struct RowTiles {
   __device__ __forceinline__ void add_masked(const f32x16 (&s)[2], int k, int hf, bool there0, bool there1, float scale) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      auto seen = [&](int r) { return (32 * k + key_of(r, hf) < limit[t]) & (r < 8 ? there0 : there1); };
+      // (against constants: sums of the lane's own cost a register each)
+      const int mine = limit[t] - 32 * k - 4 * hf, lim0 = there0 ? mine : 0, lim1 = there1 ? mine : 0;
+      auto seen = [&](int r) { return key_of(r, 0) < (r < 8 ? lim0 : lim1); };
       float mx = -INFINITY, part[4] = {};
 #pragma unroll
       for (int r = 0; r < 16; ++r) mx = fmaxf(mx, seen(r) ? s[t][r] * scale : -INFINITY);
@@ -533,163 +496,35 @@ struct RowTiles {
       l[t] += (part[0] + part[1]) + (part[2] + part[3]);
     }
   }
-  __device__ __forceinline__ void store(const PromptMass& a, int h, int part, int lane) const {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const float mo = __shfl_xor(m[t], 32, 64), lo = __shfl_xor(l[t], 32, 64);
-      const float M = fmaxf(m[t], mo), to = M == -INFINITY ? 0.f : -M;
-      const float L = l[t] * __builtin_amdgcn_exp2f(m[t] + to) + lo * __builtin_amdgcn_exp2f(mo + to);
-      const int64_t at = (tile + t) * 32 + (lane & 31);
-      if (lane < 32 && (t == 0 || second)) {
-        if (a.parts == 1) {
-          a.lse[h * a.tiles * 32 + at] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
-        } else {
-          float* ml = a.part_ml + ((h * (int64_t)a.parts + part) * a.tiles * 32 + at) * 2;
-          ml[0] = M;
-          ml[1] = L;
-        }
-      }
-    }
+  // a row's reference point and sum (both lane halves have part of it)
+  __device__ __forceinline__ float2 total(int t) const {
+    const float mo = __shfl_xor(m[t], 32, 64), lo = __shfl_xor(l[t], 32, 64);
+    const float M = fmaxf(m[t], mo), to = M == -INFINITY ? 0.f : -M;
+    return {M, l[t] * __builtin_amdgcn_exp2f(m[t] + to) + lo * __builtin_amdgcn_exp2f(mo + to)};
   }
 };
-
-// Many rows: a workgroup's four waves have 64 each and share a stream of keys.
-// grid (kv heads, row blocks x parts of the keys, sequences)
-template <int D>
-__global__ __launch_bounds__(256, 2) void prompt_rows_kernel(PromptMass a) {
-  constexpr int J = D / 16, PIECES = D / 64, TILE = 32 * D;  // 1 KiB pieces of a tile that a wave copies
-  __shared__ __attribute__((aligned(16))) uint16_t stage[3][2 * TILE];
-  const int h = blockIdx.x, b = blockIdx.z;
-  const PromptSeq sq = prompt_seq(a, b);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hf = lane >> 5;
-  const int part = blockIdx.y % a.parts;
-  // the rows that see most first
-  const int last_group = ((sq.n_rows + 63) >> 6) - 1 - (int)(blockIdx.y / a.parts) * 4, group = last_group - wave;
-  if (last_group < 0) return;  // uniform for the workgroup; a wave without rows of its own still copies
-  RowTiles<D> x;
-  x.load(a, sq, h, group, lane, part == 0);
-  // pairs of 32-key tiles
-  const int pairs = (RowTiles<D>::seen_by(a, sq, last_group) + 63) >> 6, share = (pairs + a.parts - 1) / a.parts;
-  const int k0 = part * share, k1 = min(k0 + share, (x.most + 63) >> 6);
-  const int32_t* row = a.pg.table + (int64_t)b * a.pg.table_stride;
-  const int last_tile = max((sq.kv + 15) / 16 - 1, 0);
-  bool holes = false;  // a page of the part is not there
-  for (int t = 4 * k0 + lane; t < min(4 * (k0 + share), last_tile + 1); t += 64) {
-    bool there;
-    tile_in<D>(a.pg, row[block_of(a.pg, t)], t, h, there);
-    holes |= !there;
-  }
-  holes = __any(holes);
-
-  // this wave's part of the stream's next pair (a 16-token page tile of each 32, half of it), and the ids of the blocks behind that: a table entry is
-  // read a step before the address that needs it
-  u32x4 next[2][PIECES];
-  int32_t ids[2];
-  auto page_tile = [&](int k, int i) { return min(4 * k + 2 * i + (wave >> 1), last_tile); };
-  auto look_up = [&](int k) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) ids[i] = entry(row, block_of(a.pg, page_tile(k, i)));
-  };
-  auto request = [&](int k) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      bool there;
-      const uint16_t* p = a.kc + tile_in<D>(a.pg, ids[i], page_tile(k, i), h, there) + (wave & 1) * PIECES * 512 + lane * 8;
-#pragma unroll
-      for (int j = 0; j < PIECES; ++j) next[i][j] = *reinterpret_cast<const u32x4*>(p + j * 512);
-    }
-    look_up(k + 1);
-  };
-  auto put = [&](int slot) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < PIECES; ++j) *reinterpret_cast<u32x4*>(&stage[slot][i * TILE + (wave * PIECES + j) * 512 + lane * 8]) = next[i][j];
-  };
-  const uint16_t* const keys = &stage[0][(lane & 16 ? 16 * D : 0) + (hf * 16 + (lane & 15)) * 8];
-  auto fragment = [&](int slot, int i, int j) __attribute__((always_inline)) {
-    return *reinterpret_cast<const u32x4*>(keys + slot * (2 * TILE) + i * TILE + (j >> 1) * 512 + (j & 1) * 256);
-  };
-  auto multiply = [&](int slot, int i, f32x16 (&s)[2]) __attribute__((always_inline)) {
-    u32x4 K[J];
-#pragma unroll
-    for (int j = 0; j < J; ++j) K[j] = fragment(slot, i, j);
-    x.multiply(K, s);
-  };
-  // a tile that all rows see whole: its powers, with the products of the next one (tile i of the pair in next_slot) among them
-  auto step_plain = [&](const f32x16 (&s)[2], f32x16 (&next_s)[2], int next_slot, int i) __attribute__((always_inline)) {
-    float sum[2][4];
-    multiply_among<J>([&](int j) { return fragment(next_slot, i, j); },
-                      [&](int t, int j, const u32x4& K) {
-                        next_s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(K), as_frag(x.Q[t][j]), j == 0 ? f32x16{} : next_s[t], 0, 0, 0);
-                      },
-                      [&](int t, int r) { return __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale_log2e, x.shift[t])); },
-                      [&](int t, int r, float e) { sum[t][r & 3] = r < 4 ? e : sum[t][r & 3] + e; });
-#pragma unroll
-    for (int t = 0; t < 2; ++t) x.add_plain(t, s[t], (sum[t][0] + sum[t][1]) + (sum[t][2] + sum[t][3]), a.scale_log2e);
-  };
-  if (share > 0) {
-    int k = k0, at = 0, to = 2;  // pair k's buffer, pair k + 2's
-    auto advance = [&]() __attribute__((always_inline)) {
-      put(to);
-      request(k + 3);
-    };
-    auto done = [&]() __attribute__((always_inline)) {
-      pair_done();
-      ++k;
-      at = after(at);
-      to = after(to);
-    };
-    look_up(k0);
-    request(k0);
-    put(0);
-    request(k0 + 1);
-    put(1);
-    request(k0 + 2);
-    pair_done();
-    const int plain = holes ? k0 : max(min(x.all >> 6, k1), k0);
-    if (k < plain) {
-      f32x16 s[2][2];
-      multiply(at, 0, s[0]);
-      do {
-        advance();
-        step_plain(s[0], s[1], at, 1);
-        step_plain(s[1], s[0], after(at), 0);
-        done();
-      } while (k < plain);
-    }
-    while (k < k0 + share) {
-      advance();
-      if (k < k1) {
-#pragma unroll 1
-        for (int i = 0; i < 2; ++i) {
-          f32x16 s[2];
-          multiply(at, i, s);
-          bool there0, there1;
-          tile_at<D>(a.pg, row, min(4 * k + 2 * i, last_tile), h, there0);
-          tile_at<D>(a.pg, row, min(4 * k + 2 * i + 1, last_tile), h, there1);
-          x.add_masked(s, 2 * k + i, hf, there0, there1, a.scale_log2e);
-        }
-      }
-      done();
-    }
-  }
-  if (group >= 0) x.store(a, h, part, lane);
+__device__ __forceinline__ void store_row(const PromptMass& a, int h, int part, int64_t at, float2 ml) {
+  if (a.parts == 1) a.lse[h * a.tiles * 32 + at] = ml.y == 0.f ? INFINITY : ml.x + __builtin_amdgcn_logf(ml.y);
+  else reinterpret_cast<float2*>(a.part_ml)[(h * (int64_t)a.parts + part) * a.tiles * 32 + at] = ml;
 }
 
-// Few rows (up to 192 of a sequence and kv head): nothing to share a stream of keys with.  A wave has 64 rows and a part of the keys, whose fragments
-// come straight from the cache, a tile ahead.  grid (kv heads, row groups x blocks of 4 parts, sequences)
+// A workgroup has 64 rows and its waves every fourth key tile of a part of the keys, whose fragments come straight from the cache, a tile ahead; the
+// waves join in LDS.  Three waves share a SIMD's matrix core (two: 699 us against 616 for 8192 rows of 64 heads on 8, 122 against 108 for 4 x 2048 of 32;
+// keys by way of LDS, shared by four waves of 64 rows, with the products of a tile written among the powers of the one before: 613 and 113).
+// grid (kv heads, row groups x parts of the keys, sequences)
 template <int D>
-__global__ __launch_bounds__(256, 2) void prompt_few_rows_kernel(PromptMass a) {
+__global__ __launch_bounds__(256, 3) void prompt_rows_kernel(PromptMass a) {
   constexpr int J = D / 16;
+  __shared__ float2 sm[4][64];
   const int h = blockIdx.x, b = blockIdx.z;
   const PromptSeq sq = prompt_seq(a, b);
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hf = lane >> 5;
-  const int blocks = a.parts / 4, part = (blockIdx.y % blocks) * 4 + wave, group = blockIdx.y / blocks;
-  if (group * 64 >= sq.n_rows) return;
+  // the rows that see most first
+  const int part = blockIdx.y % a.parts, group = ((sq.n_rows + 63) >> 6) - 1 - (int)(blockIdx.y / a.parts);
+  if (group < 0) return;  // uniform for the workgroup
   RowTiles<D> x;
-  x.load(a, sq, h, group, lane, part == 0);
-  const int tiles = (x.most + 31) >> 5, share = (tiles + a.parts - 1) / a.parts, k0 = part * share, k1 = min(k0 + share, tiles);
+  x.load(a, sq, h, group, lane, part == 0 && wave == 0);
+  const int tiles = (x.most + 31) >> 5, share = (tiles + a.parts - 1) / a.parts, k1 = min((part + 1) * share, tiles);
   const int32_t* row = a.pg.table + (int64_t)b * a.pg.table_stride;
   const int last_tile = max((sq.kv + 15) / 16 - 1, 0);
   struct Tile {
@@ -706,21 +541,45 @@ __global__ __launch_bounds__(256, 2) void prompt_few_rows_kernel(PromptMass a) {
   auto add = [&](int k, const Tile& t) __attribute__((always_inline)) {
     f32x16 s[2];
     x.multiply(t.K, s);
-    x.add_masked(s, k, hf, t.there0, t.there1, a.scale_log2e);
+    if (t.there0 && t.there1 && 32 * k + 32 <= x.all) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float sum[4] = {};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[r & 3] += __builtin_amdgcn_exp2f(fmaf(s[i][r], a.scale_log2e, x.shift[i]));
+        x.add_plain(i, s[i], (sum[0] + sum[1]) + (sum[2] + sum[3]), a.scale_log2e);
+      }
+    } else {
+      x.add_masked(s, k, hf, t.there0, t.there1, a.scale_log2e);
+    }
   };
-  if (k0 < k1) {
+  int k = part * share + wave;
+  if (k < k1) {
     Tile A, B;
-    load(k0, A);
-    for (int k = k0;; k += 2) {
-      load(min(k + 1, k1 - 1), B);
+    load(k, A);
+    while (true) {
+      load(min(k + 4, k1 - 1), B);
       add(k, A);
-      if (k + 1 >= k1) break;
-      load(min(k + 2, k1 - 1), A);
-      add(k + 1, B);
-      if (k + 2 >= k1) break;
+      if ((k += 4) >= k1) break;
+      load(min(k + 4, k1 - 1), A);
+      add(k, B);
+      if ((k += 4) >= k1) break;
     }
   }
-  x.store(a, h, part, lane);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const float2 ml = x.total(t);
+    if (lane < 32) sm[wave][t * 32 + lane] = ml;
+  }
+  __syncthreads();
+  if (wave != 0 || (lane >= 32 && !x.second)) return;
+  float M = -INFINITY, L = 0.f;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) M = fmaxf(M, sm[w][lane].x);
+  const float to = M == -INFINITY ? 0.f : -M;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) L += sm[w][lane].y * __builtin_amdgcn_exp2f(sm[w][lane].x + to);
+  store_row(a, h, part, x.tile * 32 + lane, {M, L});
 }
 
 __global__ __launch_bounds__(256) void prompt_join_kernel(PromptMass a) {
@@ -747,176 +606,143 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(PromptMass a) {
   a.lse[h * a.tiles * 32 + at] = L == 0.f ? INFINITY : M + __builtin_amdgcn_logf(L);
 }
 
-// The column sums.  A wave: 64 keys; the workgroup's 256 share a stream of the rows that see one of them, or of a part of those.
-// grid (kv heads, key blocks x row parts, sequences)
+// ---- the column sums: a wave's 64 keys, two tiles of 32
 template <int D>
-__global__ __launch_bounds__(256, 2) void prompt_columns_kernel(PromptMass a) {
-  constexpr int J = D / 16, TILE = 32 * D, PIECES = D / 64;
-  __shared__ __attribute__((aligned(16))) uint16_t stage[3][2 * TILE];
-  __shared__ float sm[4][64];
-  const int h = blockIdx.x, b = blockIdx.z;
-  const PromptSeq sq = prompt_seq(a, b);
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), hf = lane >> 5;
-  const int key_blocks = (a.pg.cap + 255) >> 8, block0 = (int)(blockIdx.y % key_blocks) * 256, row_part = blockIdx.y / key_blocks;
-  const int key0 = block0 + wave * 64;
-  if (block0 >= sq.kv) return;  // uniform for the workgroup
-  const int32_t* row = a.pg.table + (int64_t)b * a.pg.table_stride;
-  const int last_tile = (sq.kv + 15) / 16 - 1;
+struct Keys {
+  static constexpr int J = D / 16;
   u32x4 K[2][J];
-  bool there[4];
+  bool there[4];  // 16-token page tiles
+  bool whole;     // all of them, and all tokens in the context
+  f32x16 sum[2];
+  __device__ __forceinline__ void load(const PromptMass& a, const PromptSeq& sq, int b, int h, int key0, int lane) {
+    const int32_t* row = a.pg.table + (int64_t)b * a.pg.table_stride;
+    const int last_tile = (sq.kv + 15) / 16 - 1;
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    // 32 keys as the A operand: lane (half, t) has dims 16 j + 8 half .. + 7 of token t
-    const int k = key0 / 16 + 2 * t;
-    const int64_t at0 = tile_at<D>(a.pg, row, min(k, last_tile), h, there[2 * t]);
-    const int64_t at1 = tile_at<D>(a.pg, row, min(k + 1, last_tile), h, there[2 * t + 1]);
-    const uint16_t* p = a.kc + ((lane & 16) ? at1 : at0) + (hf * 16 + (lane & 15)) * 8;
+    for (int t = 0; t < 2; ++t) {
+      // 32 keys as the A operand: lane (half, t) has dims 16 j + 8 half .. + 7 of token t
+      const int k = key0 / 16 + 2 * t;
+      const int64_t at0 = tile_at<D>(a.pg, row, min(k, last_tile), h, there[2 * t]);
+      const int64_t at1 = tile_at<D>(a.pg, row, min(k + 1, last_tile), h, there[2 * t + 1]);
+      const uint16_t* p = a.kc + ((lane & 16) ? at1 : at0) + ((lane >> 5) * 16 + (lane & 15)) * 8;
 #pragma unroll
-    for (int j = 0; j < J; ++j) K[t][j] = *reinterpret_cast<const u32x4*>(p + (j >> 1) * 512 + (j & 1) * 256);
+      for (int j = 0; j < J; ++j) K[t][j] = *reinterpret_cast<const u32x4*>(p + (j >> 1) * 512 + (j & 1) * 256);
+      sum[t] = f32x16{};
+    }
+    whole = there[0] && there[1] && there[2] && there[3] && key0 + 64 <= sq.kv;
   }
-  const bool whole = there[0] && there[1] && there[2] && there[3] && key0 + 64 <= sq.kv;
-  f32x16 sum[2] = {{}, {}};
-  // row tiles: from the first that has a row which sees the workgroup's (the wave's) first key; from the first all of whose rows see all of
-  // the wave's keys
-  const int tiles = (sq.n_rows + 31) >> 5;
-  auto sees = [&](int key) { return (int)min((int64_t)max(key - sq.first, 0) * a.G, (int64_t)sq.n_rows); };
-  const int first = sees(block0) >> 5, share = (max(tiles - first, 0) + a.row_parts - 1) / a.row_parts;
-  const int i0 = min(first + row_part * share, tiles), i1 = min(i0 + share, tiles);
-  const int wave_first = key0 < sq.kv ? sees(key0) >> 5 : tiles, plain_from = whole ? (sees(key0 + 63) + 31) >> 5 : tiles;
-  const uint16_t* const packed = a.packed + (h * a.tiles + sq.tile0) * TILE + wave * PIECES * 512 + lane * 8;
-  const float* const lses = a.lse + (h * a.tiles + sq.tile0) * 32 + (lane & 31);
-  u32x4 next[2][PIECES];
-  float lse[4][2];  // of the rows of pairs i .. i + 3
-  auto request = [&](int i) __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int t = min(i + u, i1 - 1);
-#pragma unroll
-      for (int p = 0; p < PIECES; ++p) next[u][p] = *reinterpret_cast<const u32x4*>(packed + (int64_t)t * TILE + p * 512);
-      lse[3][u] = lses[t * 32];
-    }
-  };
-  auto put = [&](int slot) __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-#pragma unroll
-      for (int p = 0; p < PIECES; ++p) *reinterpret_cast<u32x4*>(&stage[slot][u * TILE + (wave * PIECES + p) * 512 + lane * 8]) = next[u][p];
-      lse[0][u] = lse[1][u], lse[1][u] = lse[2][u], lse[2][u] = lse[3][u];
-    }
-  };
-  auto fragment = [&](int slot, int u, int j) __attribute__((always_inline)) {
-    return *reinterpret_cast<const u32x4*>(&stage[slot][u * TILE + j * 512 + lane * 8]);
-  };
-  auto multiply = [&](int slot, int u, f32x16 (&s)[2]) __attribute__((always_inline)) {
-    s[0] = f32x16{};
-    s[1] = f32x16{};
-#pragma unroll
-    for (int j = 0; j < J; ++j) {
-      const bf16x8 Q = as_frag(fragment(slot, u, j));
-      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(K[0][j]), Q, s[0], 0, 0, 0);
-      s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(K[1][j]), Q, s[1], 0, 0, 0);
-    }
-  };
-  // rows that all see the wave's keys (or none: their sum is infinite), with the products of the next ones (tile v of the pair in next_slot) among
-  // their powers
-  auto step_plain = [&](const f32x16 (&s)[2], float log_sum, f32x16 (&next_s)[2], int next_slot, int v) __attribute__((always_inline)) {
-    multiply_among<J>([&](int j) { return fragment(next_slot, v, j); },
-                      [&](int t, int j, const u32x4& Q) {
-                        next_s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(K[t][j]), as_frag(Q), j == 0 ? f32x16{} : next_s[t], 0, 0, 0);
-                      },
-                      [&](int t, int r) { return __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale_log2e, -log_sum)); },
-                      [&](int t, int r, float e) { sum[t][r] += e; });
-  };
-  auto step_masked = [&](int i, int slot, int u, float log_sum) __attribute__((always_inline)) {
-    f32x16 s[2];
-    multiply(slot, u, s);
+  // the first row that sees a key
+  static __device__ __forceinline__ int sees(const PromptMass& a, const PromptSeq& sq, int key) {
+    return (int)min((int64_t)max(key - sq.first, 0) * a.G, (int64_t)sq.n_rows);
+  }
+  // row tile i's powers, where some rows do not see all keys (the rows behind the last have an infinite sum: powers of 0)
+  __device__ __forceinline__ void add_masked(const PromptMass& a, const PromptSeq& sq, int i, const f32x16 (&s)[2], float log_sum, int key0, int lane) {
     const int rr = i * 32 + (lane & 31), limit = rr < sq.n_rows ? min(sq.first + rr / a.G + 1, sq.kv) : 0;
+    const int mine = limit - key0 - 4 * (lane >> 5);  // (against constants: sums of the lane's own cost a register each)
+    float shift = -log_sum;
+    asm volatile("" : "+v"(shift));  // (or what both kinds of powers begin with is taken ahead of the branch between them, into 32 registers)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int lim0 = there[2 * t] ? mine : 0, lim1 = there[2 * t + 1] ? mine : 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale_log2e, shift));
+        sum[t][r] += 32 * t + key_of(r, 0) < (r < 8 ? lim0 : lim1) ? p : 0.f;
+      }
+    }
+  }
+  // the sums over the lanes' rows to 64 places
+  __device__ __forceinline__ void reduce(float* to, int lane) const {
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[t][r], a.scale_log2e, -log_sum));
-        sum[t][r] += ((key0 + 32 * t + key_of(r, hf) < limit) & there[2 * t + (r >> 3)]) ? p : 0.f;
+        float v = xor_sum<1>(sum[t][r]);
+        v = xor_sum<2>(v);
+        v = xor_sum<4>(v);
+        v = xor_sum<8>(v);
+        v = xor_sum<16>(v);
+        if ((lane & 31) == 0) to[32 * t + key_of(r, lane >> 5)] = v;
       }
-  };
-  if (i1 > i0) {
-    int i = i0, at = 0, to = 2;  // the pair of tiles i and i + 1, its buffer, that of the pair two further
-    auto advance = [&]() __attribute__((always_inline)) {
-      put(to);
-      request(i + 6);
-    };
-    auto done = [&]() __attribute__((always_inline)) {
-      pair_done();
-      i += 2;
-      at = after(at);
-      to = after(to);
-    };
-    auto masked = [&]() __attribute__((always_inline)) {
-      advance();
-      if (i >= wave_first) step_masked(i, at, 0, lse[0][0]);
-      if (i + 1 >= wave_first && i + 1 < i1) step_masked(i + 1, at, 1, lse[0][1]);
-      done();
-    };
-    request(i0);
-    put(0);
-    request(i0 + 2);
-    put(1);
-    request(i0 + 4);
-    pair_done();
-    while (i < min(plain_from, i1)) masked();
-    if (i + 2 <= i1) {
-      f32x16 s[2][2];
-      multiply(at, 0, s[0]);
-      do {
-        advance();
-        step_plain(s[0], lse[0][0], s[1], at, 1);
-        step_plain(s[1], lse[0][1], s[0], after(at), 0);
-        done();
-      } while (i + 2 <= i1);
-    }
-    if (i < i1) masked();
   }
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float v = xor_sum<1>(sum[t][r]);
-      v = xor_sum<2>(v);
-      v = xor_sum<4>(v);
-      v = xor_sum<8>(v);
-      v = xor_sum<16>(v);
-      if ((lane & 31) == 0) sm[wave][32 * t + key_of(r, hf)] = v;
-    }
-  __threadfence_block();  // (the wave's own part of the array)
-  const int j = key0 + lane;
-  if (j >= sq.kv) return;
-  const float v = sm[wave][lane];
-  if (a.row_parts > 1) {
-    a.part_sum[((int64_t)(h * a.row_parts + row_part) * a.n_seqs + b) * a.pg.cap + j] = v;
-    return;
-  }
-  const float* had = a.rows.in(b, h);
-  float* now = a.rows.out(b, h);
-  if (now != nullptr && j < a.rows.len) now[j] = (j < sq.fresh && had != nullptr ? had[j] : 0.f) + v;
-}
+};
 
-__global__ __launch_bounds__(256) void prompt_add_kernel(PromptMass a) {
-  const int h = blockIdx.x, b = blockIdx.z, j = blockIdx.y * 256 + threadIdx.x;
+// A workgroup has KW times 64 keys and 4 / KW waves for each, which take every (4 / KW)-th tile of the rows from the packed copy, a tile ahead; they
+// join in LDS.  With 128 dims two waves a SIMD and two sets of row registers (three and one set: 671 us against 615 for 8192 rows of 64 heads on 8).
+// grid (kv heads, key blocks, sequences)
+template <int D, int KW>
+__global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prompt_columns_kernel(PromptMass a) {
+  constexpr int J = D / 16, TILE = 32 * D, RW = 4 / KW;
+  __shared__ float sm[4][64];
+  const int h = blockIdx.x, b = blockIdx.z;
   const PromptSeq sq = prompt_seq(a, b);
-  const float* had = a.rows.in(b, h);
-  float* now = a.rows.out(b, h);
-  if (now == nullptr || j >= sq.kv || j >= a.rows.len) return;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rw = wave % RW;
+  const int key0 = ((int)blockIdx.y * KW + wave / RW) * 64, j = key0 + lane;
+  if ((int)blockIdx.y * KW * 64 >= sq.kv) return;  // uniform for the workgroup
+  Keys<D> x;
+  x.load(a, sq, b, h, key0, lane);
+  const float *const had = a.rows.in(b, h);
+  float* const now = a.rows.out(b, h);
+  const bool mine = rw == 0 && j < sq.kv && j < a.rows.len && now != nullptr;  // the key that the lane writes
+  const float was = mine && j < sq.fresh && had != nullptr ? had[j] : 0.f;
+  // row tiles: from the first that has a row which sees a key; from the first all of whose rows see all keys
+  const int tiles = key0 < sq.kv ? (sq.n_rows + 31) >> 5 : 0;
+  const int first = x.sees(a, sq, key0) >> 5, plain_from = x.whole ? (x.sees(a, sq, key0 + 63) + 31) >> 5 : tiles;
+  const uint16_t* const packed = a.packed + (h * a.tiles + sq.tile0) * TILE + lane * 8;
+  const float* const lses = a.lse + (h * a.tiles + sq.tile0) * 32 + (lane & 31);
+  struct Rows {
+    u32x4 Q[J];
+    float lse;
+  };
+  auto load = [&](int i, Rows& r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) r.Q[j] = *reinterpret_cast<const u32x4*>(packed + (int64_t)i * TILE + j * 512);
+    r.lse = lses[i * 32];
+  };
+  auto add = [&](int i, const Rows& r) __attribute__((always_inline)) {
+    f32x16 s[2] = {{}, {}};
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(x.K[0][j]), as_frag(r.Q[j]), s[0], 0, 0, 0);
+      s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(x.K[1][j]), as_frag(r.Q[j]), s[1], 0, 0, 0);
+    }
+    if (i >= plain_from) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r_ = 0; r_ < 16; ++r_) x.sum[t][r_] += __builtin_amdgcn_exp2f(fmaf(s[t][r_], a.scale_log2e, -r.lse));
+    } else {
+      x.add_masked(a, sq, i, s, r.lse, key0, lane);
+    }
+  };
+  // From the last rows, which all keys see, to the first: workgroups that start together read the same rows at the same time, from their
+  // XCD's L2.
+  int i = tiles - 1 - rw;
+  if (i >= first) {
+    Rows A, B;
+    load(i, A);
+    while (true) {
+      load(max(i - RW, first), B);
+      add(i, A);
+      if ((i -= RW) < first) break;
+      load(max(i - RW, first), A);
+      add(i, B);
+      if ((i -= RW) < first) break;
+    }
+  }
+  x.reduce(sm[wave], lane);
+  __syncthreads();
+  if (!mine) return;
   float v = 0.f;
-  for (int p = 0; p < a.row_parts; ++p) v += a.part_sum[((int64_t)(h * a.row_parts + p) * a.n_seqs + b) * a.pg.cap + j];
-  now[j] = (j < sq.fresh && had != nullptr ? had[j] : 0.f) + v;
+#pragma unroll
+  for (int w = 0; w < RW; ++w) v += sm[wave + w][lane];
+  now[j] = was + v;
 }
 
 struct PromptPlan {
-  int max_rows, parts, groups, row_parts;
-  bool few;
+  int max_rows, parts, groups, key_waves;
   int64_t tiles;
-  size_t packed, lse, ml, sum;  // bytes
-  size_t bytes() const { return packed + lse + ml + sum; }
+  size_t packed, lse, ml;  // bytes
+  size_t bytes() const { return packed + lse + ml; }
 };
 
 PromptPlan prompt_plan(int n_seqs, int64_t n_tokens, int max_seqlen_q, int window, int n_q, int n_kv, int D, int64_t cap) {
@@ -925,20 +751,24 @@ PromptPlan prompt_plan(int n_seqs, int64_t n_tokens, int max_seqlen_q, int windo
   p.max_rows = window > 0 ? std::min(window, max_seqlen_q) : max_seqlen_q;
   p.tiles = window > 0 ? (int64_t)n_seqs * (((int64_t)p.max_rows * G + 31) / 32) : n_tokens * G / 32 + n_seqs;
   p.groups = (int)(((int64_t)p.max_rows * G + 63) / 64);
-  p.few = p.groups <= 3;
-  const int64_t units = std::max<int64_t>((int64_t)n_seqs * n_kv, 1);
-  // parts of the keys until there are two workgroups a CU (few rows: waves, in fours), of 128 keys at least
-  const int64_t blocks = p.few ? units * p.groups : units * ((p.groups + 3) / 4);
-  const int64_t want = ((p.few ? 2048 : 512) + blocks - 1) / blocks, parts = std::max<int64_t>(1, std::min<int64_t>({want, (cap + 127) / 128, 64}));
-  p.parts = (int)(p.few ? (parts + 3) / 4 * 4 : parts);
-  // parts of the rows likewise, of eight tiles at least
-  const int64_t key_blocks = units * ((cap + 255) / 256);
-  p.row_parts = (int)std::max<int64_t>(1, std::min<int64_t>({1536 / key_blocks, (int64_t)p.groups / 4, 16}));
+  const int64_t units = std::max<int64_t>((int64_t)n_seqs * n_kv, 1), blocks = units * p.groups, key_blocks = units * ((cap + 255) / 256);
+  // parts of the keys until there are two workgroups a CU, of 512 keys at least: below that their join costs more
+  p.parts = (int)std::max<int64_t>(1, std::min<int64_t>({(512 + blocks - 1) / blocks, cap / 512, 64}));
+  // four waves for 64 keys, so that the rows are split as well - except for so many keys that they fill the chip and rows so few (below 2048 of a kv
+  // head) that a wave's keys take longer to come than the rows: 64 rows of 64 heads on 8 over 32768 keys, 49 us against 62
+  p.key_waves = key_blocks >= 256 && p.groups < 32 ? 4 : 1;
   p.packed = (size_t)n_kv * p.tiles * 32 * D * 2;
   p.lse = (size_t)n_kv * p.tiles * 32 * 4;
   p.ml = p.parts > 1 ? (size_t)n_kv * p.tiles * 32 * 8 * p.parts : 0;
-  p.sum = p.row_parts > 1 ? (size_t)n_kv * p.row_parts * n_seqs * cap * 4 : 0;
   return p;
+}
+
+template <int D>
+void launch_prompt(const PromptMass& a, const PromptPlan& p, int n_kv, int n_seqs, int64_t cap, hipStream_t stream) {
+  prompt_rows_kernel<D><<<dim3(n_kv, (unsigned)(p.groups * p.parts), n_seqs), 256, 0, stream>>>(a);
+  if (p.parts > 1) prompt_join_kernel<<<dim3(n_kv, (p.groups * 64 + 255) / 256, n_seqs), 256, 0, stream>>>(a);
+  if (p.key_waves == 4) prompt_columns_kernel<D, 4><<<dim3(n_kv, (unsigned)((cap + 255) / 256), n_seqs), 256, 0, stream>>>(a);
+  else prompt_columns_kernel<D, 1><<<dim3(n_kv, (unsigned)((cap + 63) / 64), n_seqs), 256, 0, stream>>>(a);
 }
 
 // A workgroup fills a CU.  256 units and more are left whole (two halves each: 26 + 4 us against 25 for 32 sequences of 1024 tokens on 8 kv heads);
@@ -1038,8 +868,7 @@ extern "C" int mi_prompt_attn_mass(const mi_bf16* q, int64_t q_row_stride, int64
   if (!aligned16(q) || q_row_stride % 8 != 0 || !aligned16(k_cache) || !aligned16(workspace)) return MI_EINVAL;
   const PromptPlan p = prompt_plan(n_seqs, n_tokens, std::max(max_seqlen_q, 1), window, n_q_heads, n_kv_heads, head_dim, cap);
   if (ws_bytes < p.bytes()) return MI_EWORKSPACE;
-  const int64_t row_blocks = p.few ? (int64_t)p.groups * (p.parts / 4) : (int64_t)(p.groups + 3) / 4 * p.parts;
-  if (row_blocks > 65535 || (cap + 255) / 256 * p.row_parts > 65535) return MI_EUNSUPPORTED;
+  if ((int64_t)p.groups * p.parts > 65535 || (cap + 63) / 64 > 65535) return MI_EUNSUPPORTED;
   PromptMass a;
   a.q = q, a.q_stride = q_row_stride, a.kc = k_cache;
   a.pg = {block_table, table_stride, num_blocks, block_size / 16, tile_shift(block_size), (int)cap, n_kv_heads};
@@ -1049,19 +878,10 @@ extern "C" int mi_prompt_attn_mass(const mi_bf16* q, int64_t q_row_stride, int64
   a.packed = reinterpret_cast<uint16_t*>(ws);
   a.lse = reinterpret_cast<float*>(ws + p.packed);
   a.part_ml = reinterpret_cast<float*>(ws + p.packed + p.lse);
-  a.part_sum = reinterpret_cast<float*>(ws + p.packed + p.lse + p.ml);
   a.tiles = p.tiles;
-  a.n_tokens = (int)n_tokens, a.window = window, a.max_rows = std::min(p.max_rows, max_seqlen_q), a.G = G, a.parts = p.parts, a.row_parts = p.row_parts, a.n_seqs = n_seqs;
+  a.n_tokens = (int)n_tokens, a.window = window, a.max_rows = std::min(p.max_rows, max_seqlen_q), a.G = G, a.parts = p.parts;
   a.scale_log2e = scale * 1.44269504088896340736f;
-  const dim3 rg(n_kv_heads, (unsigned)row_blocks, n_seqs);
-  const dim3 cg(n_kv_heads, (unsigned)((cap + 255) / 256 * p.row_parts), n_seqs), ag(n_kv_heads, (unsigned)((cap + 255) / 256), n_seqs);
-  if (p.few && head_dim == 128) prompt_few_rows_kernel<128><<<rg, 256, 0, S(stream)>>>(a);
-  else if (p.few) prompt_few_rows_kernel<64><<<rg, 256, 0, S(stream)>>>(a);
-  else if (head_dim == 128) prompt_rows_kernel<128><<<rg, 256, 0, S(stream)>>>(a);
-  else prompt_rows_kernel<64><<<rg, 256, 0, S(stream)>>>(a);
-  if (p.parts > 1) prompt_join_kernel<<<dim3(n_kv_heads, (p.groups * 64 + 255) / 256, n_seqs), 256, 0, S(stream)>>>(a);
-  if (head_dim == 128) prompt_columns_kernel<128><<<cg, 256, 0, S(stream)>>>(a);
-  else prompt_columns_kernel<64><<<cg, 256, 0, S(stream)>>>(a);
-  if (p.row_parts > 1) prompt_add_kernel<<<ag, 256, 0, S(stream)>>>(a);
+  if (head_dim == 128) launch_prompt<128>(a, p, n_kv_heads, n_seqs, cap, S(stream));
+  else launch_prompt<64>(a, p, n_kv_heads, n_seqs, cap, S(stream));
   return check_launch();
 }
