@@ -240,19 +240,14 @@ __device__ __forceinline__ void finish(const Evict& a, int b, int mode, int ctx,
   a.evicted[2 * ro + 1] = mode == LISTED ? dropped + ctx - n : dropped;
 }
 
-// the two 16-bit values of token f % 4 of a 16-byte piece of V (dims d and d + 16) in place of those of token e of v
-__device__ __forceinline__ void patch(u32x4& v, int e, const u32x4& x, int f) {
-  const uint32_t lo = (f & 2 ? x[1] : x[0]) >> (f & 1) * 16 & 0xffffu, hi = (f & 2 ? x[3] : x[2]) >> (f & 1) * 16 & 0xffffu;
-  const uint32_t sh = (e & 1) * 16, field = 0xffffu << sh;
-  v[e >> 1] = (v[e >> 1] & ~field) | lo << sh;
-  v[2 + (e >> 1)] = (v[2 + (e >> 1)] & ~field) | hi << sh;
-}
+// of a 16-byte piece of V, which holds two dims (16 apart) of four tokens: dim `hi` of token f % 4
+__device__ __forceinline__ uint32_t value(const u32x4& x, int hi, int f) { return (f & 2 ? x[2 * hi + 1] : x[2 * hi]) >> (f & 1) * 16 & 0xffffu; }
 
 // A wave: one tile of 16 places of one kv head; places whose page and slot are the old ones are left.  K goes in the 16-byte pieces that a token is
-// in; a piece of V holds four tokens, so that a wave builds whole pieces of its tile from those of the tokens that move there and what is there
-// already.  A token's K is in D / 8 lines of the cache and its V in a quarter of a tile: what bounds this is the lines that hold a mover, not
-// the movers' bytes.  (Teams of 16 lanes with four places each, taken from the list of movers, touch the same lines: 39 us against 42 for 32
-// sequences back to 4096 tokens, 171 against 167 for 8 from 32768, and 12 against 4 for one from 1100 to 1024.)
+// in; a piece of V holds four tokens: whole where all four are replaced, else their values one by one (2 bytes; read, patched and written back
+// whole: 40 us against 35 for 32 sequences back to 4096 tokens).  A token's K is in D / 8 lines of the cache and its V in a quarter of a tile:
+// what bounds this is the lines that hold a mover, not the movers' bytes.  (16 lanes for four places, taken from the list of movers, touch the same
+// lines: 39 us, 171 against 153 for 8 sequences from 32768 tokens, and 12 against 4 for one from 1100 to 1024; four tiles a wave: 32, 159 and 7.)
 template <int DB>
 __global__ __launch_bounds__(256) void evict_move_kernel(Evict a) {
   constexpr int TILE = 512 * DB;
@@ -279,7 +274,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(Evict a) {
 #pragma unroll
     for (int kk = 0; kk < DB; ++kk) *reinterpret_cast<u32x4*>(a.kc + dst + kk * 512 + (g * 16 + c) * 8) = x[kk];
   }
-  u32x4 v[DB], y[4][DB];
+  u32x4 y[4][DB];
   int f[4];
   bool mv[4];
 #pragma unroll
@@ -292,17 +287,28 @@ __global__ __launch_bounds__(256) void evict_move_kernel(Evict a) {
 #pragma unroll
       for (int kk = 0; kk < DB; ++kk) y[e][kk] = *reinterpret_cast<const u32x4*>(a.vc + s + kk * 512 + (f[e] % 16 / 4 * 16 + c) * 8);
   }
-  if (!(mv[0] || mv[1] || mv[2] || mv[3])) return;
-  if (!(mv[0] && mv[1] && mv[2] && mv[3]))
+  uint16_t* const to_v = a.vc + dst + lane * 8;
+  if (mv[0] && mv[1] && mv[2] && mv[3]) {
 #pragma unroll
-    for (int kk = 0; kk < DB; ++kk) v[kk] = *reinterpret_cast<const u32x4*>(a.vc + dst + kk * 512 + lane * 8);
+    for (int kk = 0; kk < DB; ++kk) {
+      u32x4 v;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        v[e] = value(y[2 * e][kk], 0, f[2 * e]) | value(y[2 * e + 1][kk], 0, f[2 * e + 1]) << 16;
+        v[2 + e] = value(y[2 * e][kk], 1, f[2 * e]) | value(y[2 * e + 1][kk], 1, f[2 * e + 1]) << 16;
+      }
+      *reinterpret_cast<u32x4*>(to_v + kk * 512) = v;
+    }
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (mv[e])
 #pragma unroll
-      for (int kk = 0; kk < DB; ++kk) patch(v[kk], e, y[e][kk], f[e]);
-#pragma unroll
-  for (int kk = 0; kk < DB; ++kk) *reinterpret_cast<u32x4*>(a.vc + dst + kk * 512 + lane * 8) = v[kk];
+      for (int kk = 0; kk < DB; ++kk) {
+        to_v[kk * 512 + e] = (uint16_t)value(y[e][kk], 0, f[e]);
+        to_v[kk * 512 + 4 + e] = (uint16_t)value(y[e][kk], 1, f[e]);
+      }
 }
 
 size_t evict_ints(int64_t batch, int64_t n_kv, int64_t keep, int64_t cap) { return batch * n_kv * (2 + (keep < cap ? 3 * keep : 0)); }

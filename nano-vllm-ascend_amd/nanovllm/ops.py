@@ -307,7 +307,7 @@ def _query_rows(name: str, q, n_q_heads: int, n_kv_heads: int, D: int):
 
 def _mass_workspace(name: str, workspace, need: int, like) -> tuple[torch.Tensor, int]:
     if workspace is None:  # torch's allocator keeps it to the stream, or to the graph that is being captured
-        return torch.empty(need, dtype=torch.uint8, device=like.device), need
+        return like.new_empty(need, dtype=torch.uint8), need
     size = workspace.numel() * workspace.element_size()
     if size < need or not workspace.is_contiguous() or workspace.get_device() != like.get_device():
         _refuse(name, f"a contiguous workspace of {need} bytes on {like.device}")
@@ -335,7 +335,7 @@ def paged_attn_decode_mass(q, k_cache, v_cache, block_tables, context_lens, mass
     if n_rows != n:
         _refuse(name, f"{n_rows} rows of q for {n} sequences")
     if out is None:
-        out = torch.empty((n, n_q_heads * D), dtype=_BF16, device=q.device)
+        out = q.new_empty((n, n_q_heads * D))
     elif out.dtype is not _BF16 or not out.is_contiguous() or out.numel() != n * n_q_heads * D or out.get_device() != q.get_device():
         _refuse(name, f"out is contiguous bfloat16 [{n}, {n_q_heads * D}]")
     if n == 0:
