@@ -230,11 +230,12 @@ __global__ __launch_bounds__(CT) void evict_choose_kernel(Evict a) {
   else choose<false>(a, tk, sm, held, mass_out, origin_out, r == ro, unit);
 }
 
-// lengths and rows, once everything has read the ones before
+// lengths and rows, once everything has read the ones before.  (A row that keeps what it has is not written: a padded batch may name one twice.)
 __device__ __forceinline__ void finish(const Evict& a, int b, int mode, int ctx, int n) {
   a.lens_out[b] = mode == NOTHING ? ctx : n;
   if (mode == NOTHING) return;
   const int64_t r = a.slots[b], ro = a.slots_out[b];
+  if (mode == SAME_PLACES && r == ro) return;
   const int kept = a.evicted[2 * r], dropped = a.evicted[2 * r + 1];
   a.evicted[2 * ro] = mode == LISTED ? n : kept;
   a.evicted[2 * ro + 1] = mode == LISTED ? dropped + ctx - n : dropped;

@@ -237,23 +237,19 @@ def paged_attn_prefill_fused(qkv, q_w, eps: float, positions, cos_sin, k_cache, 
 
 
 # --------------------------------------------------------------------------- attention mass, eviction by it
-def attn_mass_shape(rows: int, n_kv_heads: int, max_len: int) -> tuple[int, int, int]:
-    """Shape of one layer's mass (float32) and origin (int32): a row per sequence, a slot per cached token and kv head."""
-    return (rows, n_kv_heads, max_len)
-
-
 def _refuse(name: str, what: str):
     raise _C.MiError(f"{name}: {what}")
 
 
-def _here(name: str, *tensors: torch.Tensor) -> int:
-    """the current device, which every one of the tensors is on"""
-    device = torch._C._cuda_getDevice() if torch.cuda.is_available() else -1
+def _here(name: str, *tensors: torch.Tensor) -> None:
+    """every one of the tensors is on the current device"""
+    device = tensors[0].get_device()
     for t in tensors:
         if t.get_device() != device or device < 0:
             require_gpu(t)
-            _refuse(name, f"a tensor on {t.device}, the current device is cuda:{device}")
-    return device
+            _refuse(name, f"tensors on cuda:{device} and {t.device}")
+    if device != torch._C._cuda_getDevice():
+        _refuse(name, f"tensors on cuda:{device}, the current device is cuda:{torch.cuda.current_device()}")
 
 
 # (the checks' messages are put together only where one is raised: a decode step makes these calls per layer)
