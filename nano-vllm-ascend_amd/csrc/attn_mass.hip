@@ -417,13 +417,13 @@ struct RowTiles {
   bool second;                       // the second tile is there
   int all, most;                     // keys that every row sees, that the last one sees
 
-  // rows group * 64 on; group -1: none
+  // rows group * 64 on, of which there is one at least
   __device__ __forceinline__ void load(const PromptMass& a, const PromptSeq& sq, int h, int group, int lane, bool pack) {
     const int hf = lane >> 5;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int r = group * 64 + t * 32 + (lane & 31);
-      const bool on = group >= 0 && r < sq.n_rows;
+      const bool on = r < sq.n_rows;
       const int token = on ? r / a.G : 0;
       limit[t] = on ? min(sq.first + token + 1, sq.kv) : 0;
       const uint16_t* p = a.q + (int64_t)(sq.q_begin + token) * a.q_stride + (int64_t)(h * a.G + (on ? r - token * a.G : 0)) * D + 8 * hf;
@@ -433,9 +433,9 @@ struct RowTiles {
     }
     tile = sq.tile0 + group * 2;
     second = group * 64 + 32 < sq.n_rows;
-    all = group >= 0 && group * 64 + 64 <= sq.n_rows ? min(sq.first + group * 64 / a.G + 1, sq.kv) : 0;
-    most = seen_by(a, sq, group);
-    if (pack && group >= 0) {
+    all = group * 64 + 64 <= sq.n_rows ? min(sq.first + group * 64 / a.G + 1, sq.kv) : 0;
+    most = max(min(sq.first + min(group * 64 + 63, sq.n_rows - 1) / a.G + 1, sq.kv), 0);
+    if (pack) {
       uint16_t* to = a.packed + (h * a.tiles + tile) * (32 * D) + lane * 8;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
@@ -443,9 +443,6 @@ struct RowTiles {
 #pragma unroll
           for (int j = 0; j < J; ++j) *reinterpret_cast<u32x4*>(to + t * (32 * D) + j * 512) = Q[t][j];
     }
-  }
-  static __device__ __forceinline__ int seen_by(const PromptMass& a, const PromptSeq& sq, int group) {
-    return group < 0 ? 0 : max(min(sq.first + min(group * 64 + 63, sq.n_rows - 1) / a.G + 1, sq.kv), 0);
   }
   // The reference point only has to be near the maximum (32 bits hold sums of up to 2^8 as they do those of up to 1), and a sum of 16 powers tells
   // whether it is: no maximum is taken while the sums stay below.  Infinite until a key was seen, so that the first one comes here.
@@ -634,7 +631,7 @@ struct Keys {
   static __device__ __forceinline__ int sees(const PromptMass& a, const PromptSeq& sq, int key) {
     return (int)min((int64_t)max(key - sq.first, 0) * a.G, (int64_t)sq.n_rows);
   }
-  // row tile i's powers, where some rows do not see all keys (the rows behind the last have an infinite sum: powers of 0)
+  // row tile i's powers, where some rows do not see all keys or are behind the last
   __device__ __forceinline__ void add_masked(const PromptMass& a, const PromptSeq& sq, int i, const f32x16 (&s)[2], float log_sum, int key0, int lane) {
     const int rr = i * 32 + (lane & 31), limit = rr < sq.n_rows ? min(sq.first + rr / a.G + 1, sq.kv) : 0;
     const int mine = limit - key0 - 4 * (lane >> 5);  // (against constants: sums of the lane's own cost a register each)
@@ -684,9 +681,9 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prompt_columns_kernel(P
   float* const now = a.rows.out(b, h);
   const bool mine = rw == 0 && j < sq.kv && j < a.rows.len && now != nullptr;  // the key that the lane writes
   const float was = mine && j < sq.fresh && had != nullptr ? had[j] : 0.f;
-  // row tiles: from the first that has a row which sees a key; from the first all of whose rows see all keys
+  // row tiles: from the first that has a row which sees a key; those all of whose rows are there and see all keys
   const int tiles = key0 < sq.kv ? (sq.n_rows + 31) >> 5 : 0;
-  const int first = x.sees(a, sq, key0) >> 5, plain_from = x.whole ? (x.sees(a, sq, key0 + 63) + 31) >> 5 : tiles;
+  const int first = x.sees(a, sq, key0) >> 5, plain_from = x.whole ? (x.sees(a, sq, key0 + 63) + 31) >> 5 : tiles, plain_to = sq.n_rows >> 5;
   const uint16_t* const packed = a.packed + (h * a.tiles + sq.tile0) * TILE + lane * 8;
   const float* const lses = a.lse + (h * a.tiles + sq.tile0) * 32 + (lane & 31);
   struct Rows {
@@ -705,7 +702,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 3) void prompt_columns_kernel(P
       s[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(x.K[0][j]), as_frag(r.Q[j]), s[0], 0, 0, 0);
       s[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_frag(x.K[1][j]), as_frag(r.Q[j]), s[1], 0, 0, 0);
     }
-    if (i >= plain_from) {
+    if (i >= plain_from && i < plain_to) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll

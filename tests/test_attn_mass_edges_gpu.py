@@ -185,3 +185,29 @@ def test_a_query_that_is_no_number_spoils_its_own_heads_only(ops, bad):
             for h in range(hkv):
                 if (b, h) != (1, 2):
                     check_mass(got[:, h:h + 1], start[:, h:h + 1], b, b, b, new[h:h + 1], ctx, ctx - 1, bound, 310)
+
+
+def test_a_key_of_infinite_negative_score_gets_nothing(ops):
+    """... and spoils nothing: neither the other keys nor, through rows that a tile is filled up with, its own mass"""
+    gen = torch.Generator().manual_seed(10)
+    hq, hkv, d, block, ctx = 16, 8, 128, 16, 137
+    kc, vc, bt = pool(gen, hkv, d, block, [ctx])
+    kc[bt[0, 1], 3, :, 0] = float("inf")  # token 19
+    q = torch.randn(ctx, hq, d, generator=gen).bfloat16()
+    q[..., 0] = -q[..., 0].abs() - 0.5
+    k, v = device_caches(kc, vc)
+    start = torch.rand(1, hkv, 140, generator=gen)
+    finite = kc.clone()
+    finite[bt[0, 1], 3, :, 0] = 0.0
+    rows, there = ref.rows_of(finite, bt[0], ctx)
+    there[19] = False
+    for n in (1, ctx):
+        mass = start.to(DEV)
+        ops.prompt_attn_mass(q[ctx - n:].to(DEV), k, bt.to(DEV), i32(0, n), i32(ctx), n, mass, i32(0), hq, hkv, block, d ** -0.5)
+        w, A = ref.weights(q[ctx - n:], rows, there, ctx - n, d ** -0.5)
+        check_mass(mass.cpu(), start, 0, 0, 0, ref.mass_of(w, hkv), ctx, ctx - n, ref.mass_bound(d, A, ctx, 2 * n), 140)
+    mass = start.to(DEV)
+    out = ops.paged_attn_decode_mass(q[-1:].to(DEV), k, v, bt.to(DEV), i32(ctx), mass, i32(0), hq, hkv, block, d ** -0.5)
+    w, A = ref.weights(q[-1:], rows, there, ctx - 1, d ** -0.5)
+    check_mass(mass.cpu(), start, 0, 0, 0, ref.mass_of(w, hkv), ctx, ctx - 1, ref.mass_bound(d, A, ctx, 2), 140)
+    assert not bool(out.isnan().any())
