@@ -64,21 +64,26 @@ struct Counts {
   int equal[CW], n_free[CW], n_moved[CW];
 };
 
+__device__ __forceinline__ int wave_total(int v) {
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
+  return v;
+}
+
 template <bool IN_LDS>
 __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts& sm, uint32_t* held, float* mass_out, int32_t* origin_out, bool same_row,
                                        int64_t unit) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int part = ((tk.ctx + CT - 1) / CT) * 64, j0 = min(wave * part, tk.ctx), j1 = min(j0 + part, tk.ctx);
   auto key = [&](int j) { return IN_LDS ? held[j] : tk.key(j); };
-  // f(slot, key, the slot is there) for the wave's part; four keys are on their way at a time
-  auto walk = [&](auto&& f) __attribute__((always_inline)) {
-    for (int j = j0 + lane; j - lane < j1; j += 256) {
+  // f(slot, key, the slot is there) for slots from .. to - 1, 64 at a time; four keys are on their way at a time
+  auto walk = [&](int from, int to, auto&& f) __attribute__((always_inline)) {
+    for (int j = from + lane; j - lane < to; j += 256) {
       uint32_t k[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) k[i] = j + 64 * i < j1 ? key(j + 64 * i) : 0u;
+      for (int i = 0; i < 4; ++i) k[i] = j + 64 * i < to ? key(j + 64 * i) : 0u;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (j - lane + 64 * i < j1) f(j + 64 * i, k[i], j + 64 * i < j1);
+        if (j - lane + 64 * i < to) f(j + 64 * i, k[i], j + 64 * i < to);
     }
   };
   if (IN_LDS) {
@@ -89,7 +94,7 @@ __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts&
       for (int i = 0; i < 8; ++i) {
         const int at = min(j + CT * i, tk.ctx - 1);
         m[i] = tk.mass[at];
-        p[i] = tk.kept > 0 ? tk.origin[min(at, tk.kept - 1)] : 0;
+        p[i] = j - tid + CT * i < tk.kept ? tk.origin[min(at, tk.kept - 1)] : 0;  // (the same answer for the whole workgroup)
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -104,7 +109,7 @@ __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts&
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
     *reinterpret_cast<uint4*>(&sm.count[4 * tid]) = uint4{0u, 0u, 0u, 0u};
     __syncthreads();
-    walk([&](int, uint32_t k, bool on) {
+    walk(j0, j1, [&](int, uint32_t k, bool on) {
       if (on && (pass == 0 || k >> (shift + bits) == prefix)) atomicAdd(&sm.count[(k >> shift & ((1u << bits) - 1)) * COPIES + (lane & (COPIES - 1))], 1u);
     });
     __syncthreads();
@@ -135,7 +140,7 @@ __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts&
   int ties = 0;
   if (!all_equal) {
     int n_equal = 0;
-    walk([&](int, uint32_t k, bool on) { n_equal += __popcll(__ballot(on && k == prefix)); });
+    walk(j0, j1, [&](int, uint32_t k, bool on) { n_equal += __popcll(__ballot(on && k == prefix)); });
     if (lane == 0) sm.equal[wave] = n_equal;
     __syncthreads();
     for (int w = 0; w < wave; ++w) ties += sm.equal[w];
@@ -149,12 +154,17 @@ __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts&
     tie += __popcll(same);
     return yes;
   };
+  // the part's slots below keep, of which those not kept become free, and those from there on, of which those kept move
+  const int mid = min(max(a.keep, j0), j1);
   int frees = 0, moves = 0, tie = ties;
-  walk([&](int j, uint32_t k, bool on) {
-    const bool kept = stays(k, on, tie);
-    frees += __popcll(__ballot(on && j < a.keep && !kept));
-    moves += __popcll(__ballot(j >= a.keep && kept));
-  });
+  if (all_equal) {  // each lane counts, and the wave adds up once
+    walk(j0, mid, [&](int, uint32_t k, bool on) { frees += on && k < prefix; });
+    walk(mid, j1, [&](int, uint32_t k, bool on) { moves += on && k >= prefix; });
+    frees = wave_total(frees), moves = wave_total(moves);
+  } else {
+    walk(j0, mid, [&](int, uint32_t k, bool on) { frees += __popcll(__ballot(on && !stays(k, on, tie))); });
+    walk(mid, j1, [&](int, uint32_t k, bool on) { moves += __popcll(__ballot(stays(k, on, tie))); });
+  }
   if (lane == 0) sm.n_free[wave] = frees, sm.n_moved[wave] = moves;
   __syncthreads();
   int at_free = 0, at_moved = 0, all = 0;
@@ -166,14 +176,18 @@ __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts&
   int32_t* const moved = a.moved + unit * a.keep;
   int32_t* const src = a.src + unit * a.keep;
   tie = ties;
-  walk([&](int j, uint32_t k, bool on) {
-    const bool kept = stays(k, on, tie), gone = on && j < a.keep && !kept, goes = j >= a.keep && kept;
-    const uint64_t all_gone = __ballot(gone), all_go = __ballot(goes);
-    if (gone) free[at_free + __popcll(all_gone & below)] = j;
-    if (goes) moved[at_moved + __popcll(all_go & below)] = j;
-    at_free += __popcll(all_gone);
-    at_moved += __popcll(all_go);
-    if (kept && j < a.keep) src[j] = j;
+  walk(j0, mid, [&](int j, uint32_t k, bool on) {
+    const bool kept = stays(k, on, tie);
+    const uint64_t gone = __ballot(on && !kept);
+    if (kept) src[j] = j;
+    else if (on) free[at_free + __popcll(gone & below)] = j;
+    at_free += __popcll(gone);
+  });
+  walk(mid, j1, [&](int j, uint32_t k, bool on) {
+    const bool kept = stays(k, on, tie);
+    const uint64_t go = __ballot(kept);
+    if (kept) moved[at_moved + __popcll(go & below)] = j;
+    at_moved += __popcll(go);
   });
   __threadfence_block();
   __syncthreads();
