@@ -60,19 +60,31 @@ constexpr int CT = 1024, CW = CT / 64, BINS = 2048, COPIES = 2;
 
 struct Counts {
   uint32_t count[BINS * COPIES];
-  uint32_t in_wave[CW], found[3];
-  int equal[CW], n_free[CW], n_moved[CW];
+  uint32_t found[3];
+  int in_wave[CW], equal[CW], n_free[CW], n_moved[CW];
 };
 
-__device__ __forceinline__ int wave_total(int v) {
-  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
-  return v;
+// the sum over lanes 0 .. the lane's own, on the VALU's lane shifts (within 16 lanes, then the last of 16 and of 32 to those behind)
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+}
+__device__ __forceinline__ int wave_total(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+// of the waves' numbers in LDS: the sum before this wave's, and of all
+__device__ __forceinline__ int before_wave(const int* of_wave, int wave, int lane, int& all) {
+  const int s = wave_scan(lane < CW ? of_wave[lane] : 0);
+  all = __builtin_amdgcn_readlane(s, CW - 1);
+  return wave > 0 ? __builtin_amdgcn_readlane(s, wave - 1) : 0;
 }
 
 template <bool IN_LDS>
 __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts& sm, uint32_t* held, float* mass_out, int32_t* origin_out, bool same_row,
                                        int64_t unit) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int part = ((tk.ctx + CT - 1) / CT) * 64, j0 = min(wave * part, tk.ctx), j1 = min(j0 + part, tk.ctx);
   auto key = [&](int j) { return IN_LDS ? held[j] : tk.key(j); };
   // f(slot, key, the slot is there) for slots from .. to - 1, 64 at a time; four keys are on their way at a time
@@ -116,14 +128,11 @@ __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts&
     // thread t: bins 2047 - 2 t and the one below, from the top
     const uint4 v = *reinterpret_cast<const uint4*>(&sm.count[(BINS - 2 - 2 * tid) * COPIES]);
     const uint32_t c[2] = {v.z + v.w, v.x + v.y};
-    uint32_t upto = c[0] + c[1];
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t o = __shfl_up(upto, d, 64);
-      if (lane >= d) upto += o;
-    }
+    uint32_t upto = wave_scan(c[0] + c[1]);
     if (lane == 63) sm.in_wave[wave] = upto;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) upto += sm.in_wave[w];
+    int all;
+    upto += before_wave(sm.in_wave, wave, lane, all);
     uint32_t before = upto - c[0] - c[1];
     if (before < need && need <= upto) {
       const int i = before + c[0] < need;
@@ -143,7 +152,8 @@ __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts&
     walk(j0, j1, [&](int, uint32_t k, bool on) { n_equal += __popcll(__ballot(on && k == prefix)); });
     if (lane == 0) sm.equal[wave] = n_equal;
     __syncthreads();
-    for (int w = 0; w < wave; ++w) ties += sm.equal[w];
+    int all;
+    ties = before_wave(sm.equal, wave, lane, all);
   }
   const uint64_t below = (1ull << lane) - 1;
   // (the ballots of a chunk; `tie`: equal keys before it)
@@ -167,11 +177,8 @@ __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts&
   }
   if (lane == 0) sm.n_free[wave] = frees, sm.n_moved[wave] = moves;
   __syncthreads();
-  int at_free = 0, at_moved = 0, all = 0;
-  for (int w = 0; w < CW; ++w) {
-    if (w < wave) at_free += sm.n_free[w], at_moved += sm.n_moved[w];
-    all += sm.n_free[w];
-  }
+  int all;
+  int at_moved = before_wave(sm.n_moved, wave, lane, all), at_free = before_wave(sm.n_free, wave, lane, all);
   int32_t* const free = a.free + unit * a.keep;
   int32_t* const moved = a.moved + unit * a.keep;
   int32_t* const src = a.src + unit * a.keep;
