@@ -185,8 +185,7 @@ __global__ __launch_bounds__(DW * 64) void decode_mass_kernel(DecodeMass a) {
     float mc = -INFINITY;
 #pragma unroll
     for (int r = 0; r < 4; ++r) mc = fmaxf(mc, fmaxf(s[0][r], s[1][r]));
-    mc = fmaxf(mc, __shfl_xor(mc, 16, 64));
-    mc = fmaxf(mc, __shfl_xor(mc, 32, 64));
+    mc = xor_max<32>(xor_max<16>(mc));
     const float mn = fmaxf(m, mc), ms = mn == -INFINITY ? 0.f : mn;
     float p[8], ps = 0.f;
 #pragma unroll
@@ -242,8 +241,7 @@ __global__ __launch_bounds__(DW * 64) void decode_mass_kernel(DecodeMass a) {
     attend(c0, A);
   }
 
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+  l = xor_sum<32>(xor_sum<16>(l));
   if (n < G) {
 #pragma unroll
     for (int j = 0; j < 2 * DB; ++j) *reinterpret_cast<f32x4*>(&sm_o[wave][n][j * 16 + 4 * g]) = acc[j];
