@@ -263,6 +263,9 @@ __device__ __forceinline__ void finish(const Evict& a, int b, int mode, int ctx,
   a.evicted[2 * ro + 1] = mode == LISTED ? dropped + ctx - n : dropped;
 }
 
+// past the caches' own order of replacement: 156 to 139 us for 8 sequences from 32768 tokens, 35 to 29 for 32 back to 4096 (16-byte pieces; single values
+// that way take longer, 168 and 40)
+__device__ __forceinline__ void store_once(u32x4 v, uint16_t* to) { __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(to)); }
 // of a 16-byte piece of V, which holds two dims (16 apart) of four tokens: dim `hi` of token f % 4
 __device__ __forceinline__ uint32_t value(const u32x4& x, int hi, int f) { return (f & 2 ? x[2 * hi + 1] : x[2 * hi]) >> (f & 1) * 16 & 0xffffu; }
 
@@ -295,7 +298,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(Evict a) {
 #pragma unroll
     for (int kk = 0; kk < DB; ++kk) x[kk] = *reinterpret_cast<const u32x4*>(p + kk * 512);
 #pragma unroll
-    for (int kk = 0; kk < DB; ++kk) *reinterpret_cast<u32x4*>(a.kc + dst + kk * 512 + (g * 16 + c) * 8) = x[kk];
+    for (int kk = 0; kk < DB; ++kk) store_once(x[kk], a.kc + dst + kk * 512 + (g * 16 + c) * 8);
   }
   u32x4 y[4][DB];
   int f[4];
@@ -320,7 +323,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(Evict a) {
         v[e] = value(y[2 * e][kk], 0, f[2 * e]) | value(y[2 * e + 1][kk], 0, f[2 * e + 1]) << 16;
         v[2 + e] = value(y[2 * e][kk], 1, f[2 * e]) | value(y[2 * e + 1][kk], 1, f[2 * e + 1]) << 16;
       }
-      *reinterpret_cast<u32x4*>(to_v + kk * 512) = v;
+      store_once(v, to_v + kk * 512);
     }
     return;
   }
