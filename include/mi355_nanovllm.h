@@ -1073,6 +1073,8 @@ int mi_xxh64_chain_blocks(const int64_t* tokens, int n_blocks, int block_size, i
  * [0, mass_rows) has no mass written; one whose row of slots is there has a mass of 0 so far.  The tokens that a step itself stored
  * have their mass set by it, older ones are added to, so a row needs no clearing when a sequence gets it; slots at or behind the
  * context are left as they are.  No sums are made with atomics: the same call gives the same bits.
+ * Sequences of one call that have tokens name different rows; where two name one, its contents are theirs in no order (nothing else
+ * is written).
  *
  * Other than the entry points above, these look at block ids: a table entry outside [0, num_blocks) is a page that is not there -
  * its tokens are masked (they get no weight), and nothing is copied from or to it.  What masked places of the cache hold (the rest of

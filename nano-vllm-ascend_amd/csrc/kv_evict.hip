@@ -55,8 +55,10 @@ struct Tokens {
 // One workgroup per (kv head, sequence): the keep-th largest key digit by digit (11, 11 and 10 bits, counts in LDS), then the lists in slot
 // order.  A wave has a contiguous part of the slots, 64 at a time, so that ranks need the waves' totals and ballots only.  Up to HELD tokens the
 // keys are kept in LDS; longer contexts are read again in each of the six walks.  Masses share their leading bits, and lanes that add to one address
-// wait for one another: two copies of the counts.  9 us for 1100 tokens, 14 for 32 sequences of some 4200, 34 for 8 of 32768 (8 kv heads): barriers
+// wait for one another: two copies of the counts.  9 us for 1100 tokens, 14 for 32 sequences of some 4200, 37 for 8 of 32768 (8 kv heads): barriers
 // and dependent reads, then the walks over the keys on one CU.
+// (Masses that change between two walks - a call that names a row twice, another stream - make the lists disagree with their counts.  What stays
+// is then anyone's guess, but every index taken from a list is held to its range.)
 constexpr int CT = 1024, CW = CT / 64, BINS = 2048, COPIES = 2;
 
 struct Counts {
@@ -194,12 +196,17 @@ __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts&
   walk(mid, j1, [&](int j, uint32_t k, bool on) {
     const bool kept = stays(k, on, tie);
     const uint64_t go = __ballot(kept);
-    if (kept) moved[at_moved + __popcll(go & below)] = j;
+    const int at = at_moved + __popcll(go & below);
+    if (kept && at < a.keep) moved[at] = j;
     at_moved += __popcll(go);
   });
   __threadfence_block();
   __syncthreads();
-  for (int i = tid; i < all; i += CT) src[free[i]] = moved[i];
+  all = min(all, a.keep);
+  for (int i = tid; i < all; i += CT) {
+    const uint32_t to = free[i];
+    if (to < (uint32_t)a.keep) src[to] = moved[i];
+  }
   __threadfence_block();
   __syncthreads();
   // what a place's mass and position are now: in place those of moved tokens, and positions that were not written down yet
@@ -207,7 +214,7 @@ __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts&
     int from[4], p[4];
     float m[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) from[i] = src[min(j + CT * i, a.keep - 1)];
+    for (int i = 0; i < 4; ++i) from[i] = min((uint32_t)src[min(j + CT * i, a.keep - 1)], (uint32_t)tk.ctx - 1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) m[i] = tk.mass[from[i]], p[i] = tk.position(from[i]);
 #pragma unroll
@@ -271,9 +278,10 @@ __device__ __forceinline__ uint32_t value(const u32x4& x, int hi, int f) { retur
 
 // A wave: one tile of 16 places of one kv head; places whose page and slot are the old ones are left.  K goes in the 16-byte pieces that a token is
 // in; a piece of V holds four tokens: whole where all four are replaced, else their values one by one (2 bytes; read, patched and written back
-// whole: 40 us against 35 for 32 sequences back to 4096 tokens).  A token's K is in D / 8 lines of the cache and its V in a quarter of a tile:
+// whole: 40 us against 35 for 32 sequences back to 4096 tokens, before store_once).  A token's K is in D / 8 lines of the cache and its V in a quarter of a tile:
 // what bounds this is the lines that hold a mover, not the movers' bytes.  (16 lanes for four places, taken from the list of movers, touch the same
-// lines: 39 us, 171 against 153 for 8 sequences from 32768 tokens, and 12 against 4 for one from 1100 to 1024; four tiles a wave: 32, 159 and 7.)
+// lines: 39 us, 171 against 153 for 8 sequences from 32768 tokens, and 12 against 4 for one from 1100 to 1024; four tiles a wave: 32, 159 and 7;
+// all before store_once.  Now 29, 139 and 4.)
 template <int DB>
 __global__ __launch_bounds__(256) void evict_move_kernel(Evict a) {
   constexpr int TILE = 512 * DB;
@@ -286,7 +294,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(Evict a) {
   const int32_t *row = a.table + (int64_t)b * a.table_stride, *row_out = a.table_out + (int64_t)b * a.table_out_stride;
   const int to = row_out[t / a.tpb];
   const int slot = 16 * t + c;
-  const int from = slot < n && mode == LISTED ? a.src[unit * a.keep + slot] : slot;
+  const int from = slot < n && mode == LISTED ? min((uint32_t)a.src[unit * a.keep + slot], (uint32_t)ctx - 1) : slot;
   const int page = slot < n ? row[from / (16 * a.tpb)] : -1;
   const bool moves = slot < n && page >= 0 && page < a.num_blocks && (from != slot || page != to);
   if (to < 0 || to >= a.num_blocks || !__any(moves)) return;
@@ -365,7 +373,7 @@ extern "C" int mi_kv_cache_evict(mi_bf16* k_cache, mi_bf16* v_cache, int64_t num
       context_lens_out == nullptr || mass == nullptr || origin == nullptr || evicted == nullptr || slots == nullptr || slots_out == nullptr ||
       workspace == nullptr)
     return MI_EINVAL;
-  if (!aligned16(k_cache) || !aligned16(v_cache)) return MI_EINVAL;
+  if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(workspace)) return MI_EINVAL;
   const int64_t most = std::min<int64_t>(keep, cap), units = (int64_t)batch * n_kv_heads;
   const int64_t blocks = ((most + 15) / 16 + 3) / 4;
   // the places below `most` have pages of their own

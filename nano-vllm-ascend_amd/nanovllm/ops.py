@@ -258,7 +258,7 @@ def _cache_of(name: str, cache, n_kv_heads: int, block_size: int):
     if cache.dim() != 4 or cache.dtype is not _BF16 or not cache.is_contiguous():
         _refuse(name, "caches are contiguous bfloat16 [blocks, kv heads, block_size / 16, 16 * head_dim]")
     blocks, heads, tiles, elems = cache.shape
-    if blocks == 0 or heads != n_kv_heads or tiles <= 0 or tiles * 16 != block_size or (elems != 16 * HEAD_DIM and elems != 16 * 64):
+    if blocks == 0 or heads == 0 or heads != n_kv_heads or tiles <= 0 or tiles * 16 != block_size or (elems != 16 * HEAD_DIM and elems != 16 * 64):
         _refuse(name, f"a cache of shape {tuple(cache.shape)} for {n_kv_heads} kv heads and blocks of {block_size}")
     return blocks, elems // 16
 

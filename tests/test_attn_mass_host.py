@@ -61,6 +61,11 @@ def test_evict_refusals(kw, code):
     assert _C.lib.mi_kv_cache_evict(*evict_args(**kw)) == code
 
 
+@pytest.mark.parametrize("off", [4, 1])
+def test_evict_refuses_a_workspace_off_16_bytes(off):
+    assert _C.lib.mi_kv_cache_evict(*evict_args(ws=P + off)) == -1
+
+
 def test_workspace_sizes():
     lib = _C.lib
     # scores of every head and token that the table has room for; 300 sequences are not split
@@ -127,6 +132,15 @@ def test_wrappers_refuse(monkeypatch, case):
         a[key] = change(a[key])
         with pytest.raises(_C.MiError):
             call(w, a)
+
+
+@pytest.mark.parametrize("which", ["decode", "prompt", "evict"])
+def test_wrappers_refuse_caches_without_heads(monkeypatch, which):
+    monkeypatch.setattr(ops, "_here", lambda *a: 0)
+    a = good()
+    a.update(k=a["k"][:, :0], v=a["v"][:, :0], mass=a["mass"][:, :0], origin=a["origin"][:, :0], hkv=0)
+    with pytest.raises(_C.MiError):
+        call(which, a)
 
 
 def test_tensors_must_be_on_the_gpu():

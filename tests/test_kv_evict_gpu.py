@@ -149,6 +149,38 @@ def test_long_contexts(ops, ctx, keep):
     run_evict(ops, 1, 64, 256, [ctx, ctx - 17], keep, 4, 60, ctx)
 
 
+@pytest.mark.parametrize("room", [5000, 40000])
+def test_a_row_named_twice_spoils_its_own_tokens_only(ops, room):
+    """sequences of one call that share a row (which a call may not do): whatever they keep, nothing but their own places is written"""
+    from nanovllm import _C
+
+    gen = torch.Generator().manual_seed(12)
+    hkv, d, block, keep, B = 2, 64, 16, 90, 3
+    width, rows = room // block, 3
+    nblk = B * width + 2
+    table = torch.arange(B * width, dtype=torch.int32).view(B, width) + 1
+    k, v = (torch.randn(nblk, hkv, 1, 16 * d, generator=gen).bfloat16().to(DEV) for _ in range(2))
+    mass = torch.rand(rows, hkv, room, generator=gen).to(DEV)
+    origin = torch.full((rows, hkv, room), -7, dtype=torch.int32, device=DEV)
+    evicted = torch.zeros(rows, 2, dtype=torch.int32, device=DEV)
+    before = [t.clone() for t in (k, v, mass, origin, evicted)]
+    need = _C.lib.mi_kv_cache_evict_workspace(B, hkv, keep, block, width)
+    space = torch.full((need + (1 << 20),), 255, dtype=torch.uint8, device=DEV)
+    lens = torch.tensor([room - 5, room - 9, room], dtype=torch.int32, device=DEV)
+    after = ops.kv_cache_evict(k, v, table.to(DEV), lens, mass, origin, evicted, torch.tensor([1, 1, 0], dtype=torch.int32, device=DEV), keep, 2, 10, block,
+                               slots_out=torch.tensor([1, 1, 1], dtype=torch.int32, device=DEV), workspace=space[:need])
+    # (tables of 5000 // 16 pages hold 4992 tokens: contexts of more are left as they are)
+    assert after.tolist() == [keep if n <= width * block else n for n in lens.tolist()]
+    assert bool((space[need:] == 255).all())
+    first = torch.zeros(nblk, dtype=torch.bool)
+    first[table[:, :-(-keep // block)].flatten().long()] = True
+    for got, was in zip((k, v), before):
+        assert torch.equal(bits(got[~first]), bits(was[~first]))
+    for got, was in zip((mass, origin, evicted), before[2:]):
+        assert torch.equal(got[[0, 2]], was[[0, 2]])
+    assert torch.equal(mass[1, :, keep:], before[2][1, :, keep:]) and bool((origin[1, :, keep:] == -7).all())
+
+
 def test_context_longer_than_its_row_stays(ops):
     k = torch.randn(8, 1, 1, 2048, device=DEV).bfloat16()
     v, was = k.clone(), k.clone()
