@@ -1119,7 +1119,9 @@ size_t mi_kv_cache_evict_workspace(int batch, int n_kv_heads, int keep, int bloc
  * block_table_out: the pages that receive the result (the same table: in place), at least ceil(min(keep, room) / block_size) entries a row.  A page that other
  * sequences share is to be replaced by a page of the sequence's own there; an entry is the entry of block_table at the same place or a
  * page that no sequence of the call reads or writes otherwise.  Shorter contexts are only copied where pages or rows differ.  A
- * sequence with a row outside [0, mass_rows), or whose context is longer than mass_len or its table, is left as it is. */
+ * sequence with a row outside [0, mass_rows), or whose context is longer than mass_len or its table, is left as it is.  A sequence of no tokens
+ * hands evicted[slots] on to its row of slots_out only if no other sequence of the call names that row, in slots or in slots_out: rows that a batch
+ * is filled up with may name those of its sequences. */
 int mi_kv_cache_evict(mi_bf16* k_cache, mi_bf16* v_cache, int64_t num_blocks, const int32_t* block_table, int64_t table_stride,
                       const int32_t* block_table_out, int64_t table_out_stride, int table_width, const int32_t* context_lens,
                       int32_t* context_lens_out, float* mass, int32_t* origin, int32_t* evicted, int64_t mass_rows, int64_t mass_len,

@@ -248,6 +248,18 @@ __global__ __launch_bounds__(CT) void evict_choose_kernel(Evict a) {
   tk.kept = min(a.evicted[2 * r], ctx), tk.dropped = a.evicted[2 * r + 1], tk.ctx = ctx, tk.sinks = a.sinks, tk.recent = a.recent;
   float* mass_out = a.mass + (ro * a.n_kv + h) * a.len;
   int32_t* origin_out = a.origin + (ro * a.n_kv + h) * a.len;
+  if (ctx == 0) {
+    // No tokens: the pair alone, and only to a row that no other sequence of the call names - rows that a batch is filled up with may name
+    // anybody's.  Here and not in the launch that writes the others': nobody reads the row, and the pair read is not written yet.
+    if (h != 0 || r == ro) return;
+    if (tid == 0) sm.found[0] = 0;
+    __syncthreads();
+    for (int i = tid; i < (int)gridDim.y; i += CT)
+      if (i != b && (a.slots[i] == ro || a.slots_out[i] == ro)) sm.found[0] = 1;
+    __syncthreads();
+    if (tid == 0 && sm.found[0] == 0) a.evicted[2 * ro] = a.evicted[2 * r], a.evicted[2 * ro + 1] = a.evicted[2 * r + 1];
+    return;
+  }
   if (ctx <= a.keep) {
     if (r != ro) {
       for (int j = tid; j < ctx; j += CT) mass_out[j] = tk.mass[j];
@@ -259,10 +271,10 @@ __global__ __launch_bounds__(CT) void evict_choose_kernel(Evict a) {
   else choose<false>(a, tk, sm, held, mass_out, origin_out, r == ro, unit);
 }
 
-// lengths and rows, once everything has read the ones before.  (A row that keeps what it has is not written: a padded batch may name one twice.)
+// lengths and rows, once everything has read the ones before.  (A row that keeps what it has is not written.)
 __device__ __forceinline__ void finish(const Evict& a, int b, int mode, int ctx, int n) {
   a.lens_out[b] = mode == NOTHING ? ctx : n;
-  if (mode == NOTHING) return;
+  if (mode == NOTHING || ctx == 0) return;
   const int64_t r = a.slots[b], ro = a.slots_out[b];
   if (mode == SAME_PLACES && r == ro) return;
   const int kept = a.evicted[2 * r], dropped = a.evicted[2 * r + 1];

@@ -380,7 +380,8 @@ def kv_cache_evict(k_cache, v_cache, block_tables, context_lens, mass, origin, e
     contexts' lengths (context_lens_out, may be context_lens).
 
     The pages that are written are the sequence's own: a page that other sequences share (a cached prefix) is replaced in
-    block_tables_out, which then receives what is kept.  slots_out likewise for the state's rows.  Head geometries of the plain cache layout
+    block_tables_out, which then receives what is kept.  slots_out likewise for the state's rows (a padded batch's sequences of no tokens may name
+    any: a row that another sequence names is left to that one).  Head geometries of the plain cache layout
     (attention_is_plain) are not served."""
     name = "kv_cache_evict"
     if slots_out is None:
