@@ -1070,9 +1070,9 @@ int mi_xxh64_chain_blocks(const int64_t* tokens, int n_blocks, int block_size, i
  *   mass [mass_rows][n_kv_heads][mass_len] fp32, one row per sequence, slot j of the row = slot j of the sequence's context.
  * slots [batch] names the row that is read, slots_out [batch] the one that is written (the same one, or a row that no sequence of
  * the call reads: a step that may be taken back leaves the old row).  A sequence whose row of slots_out is outside
- * [0, mass_rows) has no mass written; one whose row of slots is there has a mass of 0 so far.  The tokens that a step itself stored
+ * [0, mass_rows) has no mass written; one whose row of slots is outside starts from masses of 0.  The tokens that a step itself stored
  * have their mass set by it, older ones are added to, so a row needs no clearing when a sequence gets it; slots at or behind the
- * context are left as they are.  No sums are made with atomics: the same call gives the same bits.
+ * context are left as they are, and tokens at slots behind mass_len have no mass kept.  No sums are made with atomics: the same call gives the same bits.
  * Sequences of one call that have tokens name different rows; where two name one, its contents are theirs in no order (nothing else
  * is written).
  *
@@ -1099,7 +1099,9 @@ size_t mi_prompt_attn_mass_workspace(int n_seqs, int64_t n_tokens, int max_seqle
 
 /* The mass that prompt rows give: arguments as of mi_paged_attn_prefill (q [n_tokens, n_q_heads, head_dim], K of the step's tokens in
  * the cache already, row i of a sequence at position kv_len - q_len + i); of each sequence's rows the last `window` are taken, all of them
- * for window 0.  Rows of a sequence behind the first max_seqlen_q from its end are not. */
+ * for window 0.  Rows of a sequence behind the first max_seqlen_q from its end are not: with max_seqlen_q 0 none is, and the step's tokens have a
+ * mass of 0.  A window counts from the end of the step's rows; a prompt in portions whose last rows alone are to be observed is given as
+ * many of each portion's rows as are among them. */
 int mi_prompt_attn_mass(const mi_bf16* q, int64_t q_row_stride, int64_t n_tokens, const mi_bf16* k_cache, int64_t num_blocks,
                         const int32_t* block_table, int64_t table_stride, int table_width, const int32_t* cu_seqlens_q,
                         const int32_t* kv_lens, int n_seqs, int max_seqlen_q, int window, float* mass, int64_t mass_rows,

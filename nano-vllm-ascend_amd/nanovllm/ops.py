@@ -346,8 +346,10 @@ def paged_attn_decode_mass(q, k_cache, v_cache, block_tables, context_lens, mass
 def prompt_attn_mass(q, k_cache, block_tables, cu_seqlens_q, kv_lens, max_seqlen_q: int, mass, slots, n_q_heads: int, n_kv_heads: int,
                      block_size: int, scale: float, window: int = 0, slots_out=None, workspace=None) -> None:
     """The attention mass that a prefill step's rows give (operands as paged_attn_prefill's; K of the step in the cache): all of a
-    sequence's rows, or its last `window`.  Tokens that the step stored have their mass set, those cached before are added to: portions
-    of a prompt follow one another, and decode steps follow them."""
+    sequence's rows, or its last `window` (of the step's: a portion's, where a prompt comes in portions), and no more than its last max_seqlen_q.
+    Tokens that the step stored have their mass set, those cached before are added to: portions of a prompt follow one another, and decode
+    steps follow them.  To observe the last rows of a prompt in portions, give as max_seqlen_q how many of a portion's rows are among them: with 0 the
+    portion's tokens have their mass set, to 0, and nothing is observed."""
     name = "prompt_attn_mass"
     if slots_out is None:
         slots_out = slots

@@ -3,6 +3,7 @@ contexts, and the rows of a prompt that are not observed."""
 import pytest
 import torch
 
+import attn_mass_ref as ref
 from kv_layout import to_logical
 from test_attn_mass_gpu import device_caches, pool
 
@@ -64,3 +65,133 @@ def test_padded_rows_of_an_eviction_into_other_rows(ops, first):
     assert torch.equal(filled[2], want)
     for i in (0, 1, 3, 4):
         assert torch.equal(filled[i], bare[i])
+
+
+def check_rows(got, start, rows, news, ctxs, fresh, bounds):
+    """rows: (read, written) per sequence; news: the step's mass [kv heads, ctx] per sequence; everything that no token has a place in stays"""
+    n_rows, _, room = start.shape
+    touched = torch.zeros(start.shape, dtype=torch.bool)
+    for (r, out), new, ctx, f, bound in zip(rows, news, ctxs, fresh, bounds):
+        if not 0 <= out < n_rows or ctx == 0:
+            continue
+        n = min(ctx, room)
+        old = start[r, :, :n].double() if 0 <= r < n_rows else torch.zeros(new.shape[0], n).double()
+        old = torch.where(torch.arange(n) < f, old, 0.0)
+        limit = bound * new[:, :n] + ref.U * (old + new[:, :n]) + 1e-30
+        diff = (got[out, :, :n].double() - old - new[:, :n]).abs()
+        assert bool((diff <= limit).all()), (r, out, float((diff / limit).max()))
+        touched[out, :, :n] = True
+    assert torch.equal(got[~touched], start[~touched])
+
+
+# rows read and written by four sequences, of five: there, in place, none to read, none to write
+ROWS = [[(0, 1), (2, 2), (-1, 3), (5, 4)], [(0, -1), (1, 5), (2, 3), (4, 4)], [(-9, 0), (2 ** 31 - 1, 1), (2, 2 ** 31 - 1), (3, -2 ** 31)]]
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("geometry,ctxs,room", [
+    ((16, 8, 128), [200, 17, 1, 130], 205), ((16, 8, 128), [200, 17, 1, 130], 100), ((14, 2, 64), [200, 16, 201, 130], 200),   # not split
+    ((16, 8, 128), [700, 17, 1, 400], 705), ((16, 8, 128), [700, 401, 1, 400], 400), ((14, 2, 64), [1500, 300, 255, 257], 256)])
+def test_decode_rows_and_their_length(ops, rows, geometry, ctxs, room):
+    hq, hkv, d = geometry
+    gen = torch.Generator().manual_seed(room)
+    kc, vc, bt = pool(gen, hkv, d, 16, ctxs)
+    k, v = device_caches(kc, vc)
+    q = torch.randn(4, hq, d, generator=gen).bfloat16()
+    start = torch.rand(5, hkv, room, generator=gen)
+    mass = start.to(DEV)
+    ops.paged_attn_decode_mass(q.to(DEV), k, v, bt.to(DEV), dev(ctxs), mass, dev([r for r, _ in rows]), hq, hkv, 16, d ** -0.5,
+                               slots_out=dev([r for _, r in rows]))
+    news, bounds = [], []
+    for b, ctx in enumerate(ctxs):
+        w, A = ref.weights(q[b:b + 1], *ref.rows_of(kc, bt[b], ctx), ctx - 1, d ** -0.5)
+        news.append(ref.mass_of(w, hkv))
+        bounds.append(ref.mass_bound(d, A, ctx, hq // hkv))
+    check_rows(mass.cpu(), start, rows, news, ctxs, [c - 1 for c in ctxs], bounds)
+
+
+def run_prompt_rows(ops, geometry, news, pasts, rows, room, window, max_q, wider, seed):
+    """wider: entries of the tables beyond the contexts (what the form of the column sums goes by, too)"""
+    hq, hkv, d = geometry
+    gen = torch.Generator().manual_seed(seed)
+    ctxs = [n + p for n, p in zip(news, pasts)]
+    kc, vc, bt = pool(gen, hkv, d, 16, ctxs, width_more=wider)
+    k, _ = device_caches(kc, vc)
+    cu = [sum(news[:i]) for i in range(len(news) + 1)]
+    q = torch.randn(cu[-1], hq, d, generator=gen).bfloat16()
+    start = torch.rand(max(5, 2 * len(news)), hkv, room, generator=gen)
+    mass = start.to(DEV)
+    ops.prompt_attn_mass(q.to(DEV), k, bt.to(DEV), dev(cu), dev(ctxs), max_q, mass, dev([r for r, _ in rows]), hq, hkv, 16, d ** -0.5, window=window,
+                         slots_out=dev([r for _, r in rows]))
+    given, bounds = [], []
+    for b, ctx in enumerate(ctxs):
+        seen = min(news[b], max_q, window or max_q)
+        A, w = 0.0, torch.zeros(hq, 1, ctx).double()
+        if seen:
+            w, A = ref.weights(q[cu[b + 1] - seen:cu[b + 1]], *ref.rows_of(kc, bt[b], ctx), ctx - seen, d ** -0.5)
+        given.append(ref.mass_of(w, hkv))
+        bounds.append(ref.mass_bound(d, A, ctx, seen * hq // hkv))
+    check_rows(mass.cpu(), start, rows, given, ctxs, pasts, bounds)
+
+
+WIDER = [2, 200]  # 4 sequences on 8 kv heads: key blocks of one wave's keys, and with 256 blocks of four waves' and more, those
+
+
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("wider", WIDER)
+@pytest.mark.parametrize("room", [205, 150])
+def test_prompt_rows_and_their_length(ops, rows, wider, room):
+    run_prompt_rows(ops, (16, 8, 128), [60, 17, 1, 130], [140, 0, 64, 70], rows, room, 0, 130, wider, 31)
+    run_prompt_rows(ops, (32, 8, 64), [60, 17, 1, 130], [140, 0, 64, 70], rows, room, 19, 130, wider, 32)
+
+
+@pytest.mark.parametrize("max_q", [0, 1, 33, 64])
+@pytest.mark.parametrize("window", [0, 1, 40])
+@pytest.mark.parametrize("wider", WIDER)
+def test_prompt_rows_behind_the_first_max_seqlen_q_are_not_taken(ops, max_q, window, wider):
+    """counted from a sequence's end; the tokens that the step stored have their mass set all the same"""
+    rows = [(0, 1), (2, 2), (3, 4), (5, 6)]
+    run_prompt_rows(ops, (16, 8, 128), [90, 33, 5, 200], [0, 100, 20, 7], rows, 210, window, max_q, wider, 33)
+    run_prompt_rows(ops, (32, 8, 64), [90, 33, 5, 200], [0, 100, 20, 7], rows, 210, window, max_q, wider, 34)
+
+
+@pytest.mark.parametrize("wider", [2, 600])
+def test_the_last_rows_of_a_prompt_in_portions(ops, wider):
+    """max_seqlen_q = 0 sets the mass of a portion's tokens and observes nothing: the prompt's last 32 rows, however it is cut - the portion
+    before the last one observes what the last is too short for"""
+    hq, hkv, d, ctx, window = 16, 8, 128, 300, 32
+    gen = torch.Generator().manual_seed(35)
+    kc, vc, bt = pool(gen, hkv, d, 16, [ctx], width_more=wider)
+    k, _ = device_caches(kc, vc)
+    q = torch.randn(ctx, hq, d, generator=gen).bfloat16()
+    w, A = ref.weights(q[-window:], *ref.rows_of(kc, bt[0], ctx), ctx - window, d ** -0.5)
+    want, bound = ref.mass_of(w, hkv), ref.mass_bound(d, A, ctx, window * hq // hkv)
+    for cuts in ([0, 300], [0, 100, 220, 300], [0, 1, 290, 300]):
+        mass = torch.full((1, hkv, 304), float("nan"), device=DEV)  # rows need no clearing
+        for lo, hi in zip(cuts, cuts[1:]):
+            seen = max(0, hi - max(lo, ctx - window))  # of the portion's rows those among the prompt's last
+            ops.prompt_attn_mass(q[lo:hi].to(DEV), k, bt.to(DEV), dev([0, hi - lo]), dev([hi]), seen, mass, dev([0]), hq, hkv, 16, d ** -0.5)
+        got = mass[0, :, :ctx].cpu().double()
+        # (a portion more, a rounding of the sum more)
+        assert bool(((got - want).abs() <= (bound + len(cuts) * ref.U) * want + 1e-30).all())
+        assert bool(mass[0, :, ctx:].isnan().all())
+
+
+@pytest.mark.parametrize("read,written", [(-1, 1), (3, 1), (0, -1), (0, 3), (-2 ** 31, 2 ** 31 - 1)])
+@pytest.mark.parametrize("ctx", [100, 40])
+def test_eviction_with_a_row_that_is_not_there(ops, read, written, ctx):
+    """... of either kind leaves its sequence as it is, and the others are evicted"""
+    gen = torch.Generator().manual_seed(36)
+    kc, vc, bt = pool(gen, 2, 64, 16, [ctx, 90])
+    mass = torch.rand(3, 2, 104, generator=gen)
+    origin, evicted = torch.full((3, 2, 104), -5, dtype=torch.int32), torch.tensor([[9, 90], [8, 80], [0, 0]], dtype=torch.int32)
+    results = []
+    for b in (0, 1):  # with the sequence, and the other one alone
+        k, v = device_caches(kc, vc)
+        state = [t.to(DEV) for t in (mass, origin, evicted)]
+        after = ops.kv_cache_evict(k, v, bt[b:].to(DEV), dev([ctx, 90][b:]), *state, dev([read, 2][b:]), 48, 2, 10, 16, slots_out=dev([written, 2][b:]))
+        assert after.tolist() == [ctx, 48][b:]
+        results.append([t.cpu() for t in state] + [t.view(torch.int16).cpu() for t in (k, v)])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert results[0][2].tolist() == [[9, 90], [8, 80], [48, 42]]
