@@ -175,7 +175,10 @@ __device__ __forceinline__ void choose(const Evict& a, const Tokens& tk, Counts&
     walk(mid, j1, [&](int, uint32_t k, bool on) { moves += on && k >= prefix; });
     frees = wave_total(frees), moves = wave_total(moves);
   } else {
-    walk(j0, mid, [&](int, uint32_t k, bool on) { frees += __popcll(__ballot(on && !stays(k, on, tie))); });
+    walk(j0, mid, [&](int, uint32_t k, bool on) {  // (stays() in every lane, those behind `mid` too: it counts the equal keys for what follows)
+      const bool kept = stays(k, on, tie);
+      frees += __popcll(__ballot(on && !kept));
+    });
     walk(mid, j1, [&](int, uint32_t k, bool on) { moves += __popcll(__ballot(stays(k, on, tie))); });
   }
   if (lane == 0) sm.n_free[wave] = frees, sm.n_moved[wave] = moves;

@@ -314,3 +314,35 @@ def test_a_sequence_on_a_budget(ops):
             evict()
             check_state()
     check_state()
+
+
+@pytest.mark.parametrize("ctx,block", [(1500, 16), (3000, 64), (12000, 64), (32768, 256), (33000, 256)])
+@pytest.mark.parametrize("keep", [36, 63, 100, 163, 700, 1000])
+def test_equal_masses_around_a_budget_off_64_slots(ops, ctx, block, keep):
+    """The last of the equal masses that stay is in the 64 slots that the budget cuts.  First sequence: all slots below the budget and those from
+    the budget's own place in the next 64 on are equal, and two behind are larger; the others: masses of two kinds, of one, and zero or not"""
+    gen = torch.Generator().manual_seed(ctx + keep)
+    hkv, d = 2, 64
+    mass = torch.zeros(4, hkv, ctx)
+    mass[0, :, :keep] = 1.0
+    mass[0, :, keep + keep % 64:keep + 64] = 1.0
+    mass[0, :, [ctx - 20, ctx - 1]] = 2.0
+    mass[1] = torch.randint(0, 2, (hkv, ctx), generator=gen)
+    mass[2] = 0.5
+    mass[3] = torch.rand(hkv, ctx, generator=gen) * (torch.rand(hkv, ctx, generator=gen) < keep / ctx / 2)
+    per = -(-ctx // block)
+    bt = torch.randperm(4 * per, generator=gen).view(4, per).to(torch.int32)
+    kc = torch.randn(4 * per, block, hkv, d, generator=gen).bfloat16()
+    k, v = to_fragment(kc, False).to(DEV), to_fragment(kc, True).to(DEV)
+    m, origin = mass.to(DEV), torch.zeros(4, hkv, ctx, dtype=torch.int32, device=DEV)
+    evicted, slots = torch.zeros(4, 2, dtype=torch.int32, device=DEV), torch.arange(4, dtype=torch.int32, device=DEV)
+    ops.kv_cache_evict(k, v, bt.to(DEV), torch.full((4,), ctx, dtype=torch.int32, device=DEV), m, origin, evicted, slots, keep, 0, 0, block)
+    got_k, got_v = to_logical(k.cpu(), block, False), to_logical(v.cpu(), block, True)
+    i = torch.arange(keep)
+    for b in range(4):
+        for h in range(hkv):
+            src = torch.tensor(ref.choose(mass[b, h], torch.arange(ctx), ctx, keep, 0, 0))
+            assert torch.equal(origin[b, h, :keep].cpu().long(), src), (b, h)
+            assert torch.equal(m[b, h, :keep].cpu(), mass[b, h][src])
+            for got in (got_k, got_v):
+                assert torch.equal(bits(got[bt[b, i // block].long(), i % block, h]), bits(kc[bt[b, src // block].long(), src % block, h]))
