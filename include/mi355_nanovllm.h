@@ -1120,7 +1120,8 @@ size_t mi_kv_cache_evict_workspace(int batch, int n_kv_heads, int keep, int bloc
  *
  * block_table_out: the pages that receive the result (the same table: in place), at least ceil(min(keep, room) / block_size) entries a row.  A page that other
  * sequences share is to be replaced by a page of the sequence's own there; an entry is the entry of block_table at the same place or a
- * page that no sequence of the call reads or writes otherwise.  Shorter contexts are only copied where pages or rows differ.  A
+ * page that no sequence of the call reads or writes otherwise.  Shorter contexts are only copied where pages or rows differ.  Which tokens stay does not
+ * depend on whether their pages are there; the place of one whose page is not holds what it held.  A
  * sequence with a row outside [0, mass_rows), or whose context is longer than mass_len or its table, is left as it is.  A sequence of no tokens
  * hands evicted[slots] on to its row of slots_out only if no other sequence of the call names that row, in slots or in slots_out: rows that a batch
  * is filled up with may name those of its sequences. */

@@ -72,8 +72,8 @@ struct MassRows {
 // scores go out in 32 bits on the way (64-byte pieces per head and tile).  The waves join in LDS.  With one split the workgroup
 // then reads its scores back (they are in its XCD's L2) and adds the weights; with more a second launch joins the splits, too.
 //
-// Bound by HBM: 208 us for 8 contexts of 32768 tokens, 64 heads of 128 on 8 (1.16 GB with the scores: 5.6 TB/s) and 18 for the join (84 MB),
-// 25 us for 32 x 1024 of 16 heads on 8 (5.5 TB/s), 54 + 8 for one of 131072 of 32 heads of 64 on 8 (5.3 TB/s).
+// Bound by HBM: 208 us for 8 contexts of 32768 tokens, 64 heads of 128 on 8 (K, V, the scores and the splits' sums, 1.145 GB: 5.5 TB/s) and 18 for
+// the join (84 MB), 24 us for 32 x 1024 of 16 heads on 8 (138 MB: 5.7 TB/s), 54 + 8 for one of 131072 of 32 heads of 64 on 8 (285 MB: 5.3 TB/s).
 // ---------------------------------------------------------------------------------------------------------------------
 struct DecodeMass {
   const uint16_t* q;
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(256) void decode_mass_join_kernel(DecodeMass a) {
 // neither the running maximum and sum nor the column sums leave the lane before the end.
 //
 // Bound by the matrix cores at the clock that random operands leave them, and the powers beside them (a score: 8 cycles of matrix instruction,
-// 16 of fma, exp2 and sum): 250 us each walk for 4096 rows of 32 heads on 8 behind 4096 tokens (206 GFLOP: 825 TFLOP/s), 49 + 48 for the last 64
+// 16 of fma, exp2 and sum): 240 us each walk for 4096 rows of 32 heads on 8 behind 4096 tokens (206 GFLOP: 860 TFLOP/s), 47 + 47 for the last 64
 // rows of 64 heads over 32768; and by launches and dependent reads for short ones, 6 + 7 us for 137 rows.
 // ---------------------------------------------------------------------------------------------------------------------
 struct PromptMass {
@@ -773,8 +773,9 @@ void launch_prompt(const PromptMass& a, const PromptPlan& p, int n_kv, int n_seq
   else prompt_columns_kernel<D, 1><<<dim3(n_kv, (unsigned)((cap + 63) / 64), n_seqs), 256, 0, stream>>>(a);
 }
 
-// A workgroup fills a CU.  256 units and more are left whole (two halves each: 26 + 4 us against 25 for 32 sequences of 1024 tokens on 8 kv heads);
-// fewer are split into some four workgroups a CU, so that contexts of all lengths share the chip evenly (24 sequences of 101 to 8000 tokens on 4
+// A workgroup fills a CU (with 64-wide heads half of one).  256 units and more are left whole, whatever the lengths of their contexts (32 sequences of
+// 1024 tokens on 8 kv heads, 128-wide: 25 us, in two halves each 26 + 4; 64-wide, 32 heads: 14 us, 73 MB at 5.3 TB/s); fewer are split into some
+// four workgroups a CU, so that contexts of all lengths share the chip evenly (24 sequences of 101 to 8000 tokens on 4
 // kv heads: 55 us with one a CU, 48 with four), of 256 tokens at least.
 int decode_splits(int batch, int n_kv, int64_t cap) {
   const int64_t units = std::max<int64_t>((int64_t)batch * n_kv, 1);

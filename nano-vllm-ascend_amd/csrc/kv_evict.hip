@@ -55,7 +55,7 @@ struct Tokens {
 // One workgroup per (kv head, sequence): the keep-th largest key digit by digit (11, 11 and 10 bits, counts in LDS), then the lists in slot
 // order.  A wave has a contiguous part of the slots, 64 at a time, so that ranks need the waves' totals and ballots only.  Up to HELD tokens the
 // keys are kept in LDS; longer contexts are read again in each of the six walks.  Masses share their leading bits, and lanes that add to one address
-// wait for one another: two copies of the counts.  9 us for 1100 tokens, 14 for 32 sequences of some 4200, 37 for 8 of 32768 (8 kv heads): barriers
+// wait for one another: two copies of the counts.  10 us for 1100 tokens, 14 for 32 sequences of some 4200, 37 for 8 of 32768 (8 kv heads): barriers
 // and dependent reads, then the walks over the keys on one CU.
 // (Masses that change between two walks - a call that names a row twice, another stream - make the lists disagree with their counts.  What stays
 // is then anyone's guess, but every index taken from a list is held to its range.)
@@ -285,7 +285,7 @@ __device__ __forceinline__ void finish(const Evict& a, int b, int mode, int ctx,
   a.evicted[2 * ro + 1] = mode == LISTED ? dropped + ctx - n : dropped;
 }
 
-// past the caches' own order of replacement: 156 to 139 us for 8 sequences from 32768 tokens, 35 to 29 for 32 back to 4096 (16-byte pieces; single values
+// past the caches' own order of replacement: 156 to 139 us for 8 sequences from 32768 tokens, 35 to 28 for 32 back to 4096 (16-byte pieces; single values
 // that way take longer, 168 and 40)
 __device__ __forceinline__ void store_once(u32x4 v, uint16_t* to) { __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(to)); }
 // of a 16-byte piece of V, which holds two dims (16 apart) of four tokens: dim `hi` of token f % 4
@@ -296,7 +296,7 @@ __device__ __forceinline__ uint32_t value(const u32x4& x, int hi, int f) { retur
 // whole: 40 us against 35 for 32 sequences back to 4096 tokens, before store_once).  A token's K is in D / 8 lines of the cache and its V in a quarter of a tile:
 // what bounds this is the lines that hold a mover, not the movers' bytes.  (16 lanes for four places, taken from the list of movers, touch the same
 // lines: 39 us, 171 against 153 for 8 sequences from 32768 tokens, and 12 against 4 for one from 1100 to 1024; four tiles a wave: 32, 159 and 7;
-// all before store_once.  Now 29, 139 and 4.)
+// all before store_once.  Now 28, 141 and 4.)
 template <int DB>
 __global__ __launch_bounds__(256) void evict_move_kernel(Evict a) {
   constexpr int TILE = 512 * DB;

@@ -195,3 +195,27 @@ def test_eviction_with_a_row_that_is_not_there(ops, read, written, ctx):
     for a, b in zip(*results):
         assert torch.equal(a, b)
     assert results[0][2].tolist() == [[9, 90], [8, 80], [48, 42]]
+
+
+def test_narrow_views_of_wide_tables(ops):
+    """rows of a table further apart than what may be used of them: the same bits as from a table of that width"""
+    gen = torch.Generator().manual_seed(37)
+    hq, hkv, d, block, ctxs = 16, 8, 128, 16, [300, 41, 170]
+    kc, vc, bt = pool(gen, hkv, d, block, ctxs, width_more=60)
+    assert bt.shape[1] == 79
+    q = torch.randn(60, hq, d, generator=gen).bfloat16().to(DEV)
+    start = torch.rand(3, hkv, 304, generator=gen)
+    results = []
+    for copied in (False, True):
+        table = bt.to(DEV)[:, :19]
+        table = table.contiguous() if copied else table
+        k, v = device_caches(kc, vc)
+        mass, lens, slots = start.to(DEV), dev(ctxs), dev([2, 0, 1])
+        origin, evicted = torch.zeros(3, hkv, 304, dtype=torch.int32, device=DEV), torch.zeros(3, 2, dtype=torch.int32, device=DEV)
+        ops.prompt_attn_mass(q, k, table, dev([0, 30, 40, 60]), lens, 30, mass, slots, hq, hkv, block, 0.1)
+        out = ops.paged_attn_decode_mass(q[:3], k, v, table, lens, mass, slots, hq, hkv, block, 0.1)
+        after = ops.kv_cache_evict(k, v, table, lens, mass, origin, evicted, slots, 100, 2, 10, block)
+        assert after.tolist() == [100, 41, 100]
+        results.append([t.cpu() for t in (out.view(torch.int16), mass, origin, evicted, k.view(torch.int16), v.view(torch.int16))])
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
